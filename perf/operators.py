@@ -369,10 +369,10 @@ def _run_attend(s):
         import chia_proj_amd as lib
 
         return lib.attention_cache(s["q"], s["kc"], s["vc"], s["ks"], s["vs"], s["table"], s["lens"],
-                               None if c["n"] == 1 else s["cu"], max_query=s["max_n"], max_seqlen=s["max_len"],
-                               norm=c.get("norm", "softmax"), causal=True, softcap=c.get("softcap", 0.0),
-                               alibi_slopes=s["slopes"], bias=s["bias"] if c.get("norm") == "sigmoid" else 0.0,
-                               **_mask(c))
+                                   None if c["n"] == 1 else s["cu"], max_query=s["max_n"], max_seqlen=s["max_len"],
+                                   norm=c.get("norm", "softmax"), causal=True, softcap=c.get("softcap", 0.0),
+                                   alibi_slopes=s["slopes"], bias=s["bias"] if c.get("norm") == "sigmoid" else 0.0,
+                                   **_mask(c))
     m = _mask(c)
     H, Hkv, D = c["H"], c["Hkv"], c["D"]
     G, lens, cu = H // Hkv, s["lens"].long(), s["cu"].long()
