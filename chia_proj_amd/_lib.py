@@ -157,6 +157,126 @@ class PlanInfo(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_ if name != "reserved"}
 
 
+# Entry points declared in include/chia_cache.h (checked by the CPU tests).
+CACHE_EXPORTS = (
+    "chia_cache_tables",
+    "chia_cache_release",
+    "chia_cache_write",
+    "chia_cache_attn_workspace_size",
+    "chia_cache_attn",
+)
+
+_i64x2 = ctypes.c_int64 * 2
+
+
+class _CacheStruct(ctypes.Structure):
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(type(self))
+        for key, val in kw.items():
+            setattr(self, key, val)
+
+
+class CacheTablesArgs(_CacheStruct):
+    """Mirror of ``chia_cache_tables_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("block_size", ctypes.c_int32),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("requests", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("context_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("free_capacity", ctypes.c_int64),
+        ("max_tokens", ctypes.c_int64),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("free_left", ctypes.c_void_p),
+        ("missing", ctypes.c_void_p),
+        ("reserved", ctypes.c_int32 * 8),
+    ]
+
+
+class CacheReleaseArgs(_CacheStruct):
+    """Mirror of ``chia_cache_release_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("block_size", ctypes.c_int32),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("requests", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("context_lens", ctypes.c_void_p),
+        ("finished", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("free_capacity", ctypes.c_int64),
+        ("free_left", ctypes.c_void_p),
+        ("reserved", ctypes.c_int32 * 8),
+    ]
+
+
+class CacheWriteArgs(_CacheStruct):
+    """Mirror of ``chia_cache_write_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("format", ctypes.c_uint32),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("k_stride", _i64x2),
+        ("v_stride", _i64x2),
+        ("k_cache_stride", _i64x3),
+        ("v_cache_stride", _i64x3),
+        ("k_scale_stride", _i64x2),
+        ("v_scale_stride", _i64x2),
+        ("block_size", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 7),
+    ]
+
+
+class CacheAttnArgs(_CacheStruct):
+    """Mirror of ``chia_cache_attn_args``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("format", ctypes.c_uint32),
+        ("attn", ctypes.POINTER(AttnArgs)),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_scale_stride", _i64x2),
+        ("v_scale_stride", _i64x2),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("queries", ctypes.c_int64),
+        ("max_query", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("reserved", ctypes.c_int32 * 8),
+    ]
+
+
 class ChiaAttnError(RuntimeError):
     """A non-zero status returned by the C ABI."""
 
@@ -211,6 +331,13 @@ def _load():
         lib.chia_attn_status_string.restype = ctypes.c_char_p
         lib.chia_attn_abi_version.argtypes = []
         lib.chia_attn_abi_version.restype = ctypes.c_int
+        for name, args in (("tables", CacheTablesArgs), ("release", CacheReleaseArgs), ("write", CacheWriteArgs),
+                           ("attn", CacheAttnArgs)):
+            fn = getattr(lib, "chia_cache_" + name)
+            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.chia_cache_attn_workspace_size.argtypes = [ctypes.POINTER(CacheAttnArgs)]
+        lib.chia_cache_attn_workspace_size.restype = ctypes.c_int64
         if lib.chia_attn_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH.name} ABI {lib.chia_attn_abi_version()} != expected {ABI_VERSION}")
         _lib = lib
@@ -262,6 +389,37 @@ def bwd_noalloc(args: BwdArgs, stream: int) -> None:
     st = _load().chia_attn_bwd_noalloc(ctypes.byref(args), ctypes.c_void_p(stream))
     if st != 0:
         raise ChiaAttnError(st, "chia_attn_bwd_noalloc")
+
+
+def cache_tables(args: CacheTablesArgs, stream: int) -> None:
+    st = _load().chia_cache_tables(args, stream)
+    if st != 0:
+        raise ChiaAttnError(st, "chia_cache_tables")
+
+
+def cache_release(args: CacheReleaseArgs, stream: int) -> None:
+    st = _load().chia_cache_release(args, stream)
+    if st != 0:
+        raise ChiaAttnError(st, "chia_cache_release")
+
+
+def cache_write(args: CacheWriteArgs, stream: int) -> None:
+    st = _load().chia_cache_write(args, stream)
+    if st != 0:
+        raise ChiaAttnError(st, "chia_cache_write")
+
+
+def cache_attn_workspace_size(args: CacheAttnArgs) -> int:
+    n = _load().chia_cache_attn_workspace_size(args)
+    if n < 0:
+        raise ChiaAttnError(int(n), "chia_cache_attn_workspace_size")
+    return int(n)
+
+
+def cache_attn(args: CacheAttnArgs, stream: int) -> None:
+    st = _load().chia_cache_attn(args, stream)
+    if st != 0:
+        raise ChiaAttnError(st, "chia_cache_attn")
 
 
 def plan(args: AttnArgs) -> dict:

@@ -1,0 +1,242 @@
+// cache_attn.hip -- chia_cache_attn: argument checks, the launch of the cache
+// attention kernels (cache_attn_kernel.h) and the kernel that joins split keys.
+#include <cmath>
+
+#include "cache_attn_kernel.h"
+#include "chia_cache.h"
+
+namespace chia {
+namespace {
+
+// Joins the parts of rows whose keys were split: o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z.
+// 32 (D = 128) or 16 lanes to a row, float4 each.
+template <int D, bool SOFTMAX, int ROWS>
+__global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnParams p) {
+  constexpr int LPR = D / 4, PER = 256 / LPR;  // lanes per row, rows at a time
+  const int rh = udiv((int)blockIdx.x, p.div_tiles), rt0 = (int)blockIdx.x - rh * p.tiles;
+  const int r = udiv(rh, p.div_hkv), hk = rh - r * p.Hkv;
+  const CacheSpan sp = cache_span(p, r);
+  const int n_rows = sp.n * p.G;
+  for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
+    const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
+    const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
+    const int used = (tw.n + chunk - 1) / chunk;
+    if (used <= 1) continue;
+    for (int i = (int)threadIdx.x / LPR; i < ROWS; i += PER) {
+      const int row = rt * ROWS + i;
+      if (row >= n_rows) break;
+      const int t = udiv(row, p.div_g), h = hk * p.G + row - t * p.G;
+      const int64_t th = (int64_t)p.T * p.H, at = (int64_t)(sp.tok0 + t) * p.H + h;
+      const int d = 4 * ((int)threadIdx.x % LPR);
+      float f = p.post_scale;
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (SOFTMAX) {
+        float m = -INFINITY, l = 0.f;
+        for (int z = 0; z < used; ++z) m = fmaxf(m, p.part_ml[2 * (z * th + at)]);
+        for (int z = 0; z < used; ++z) {
+          const float mz = p.part_ml[2 * (z * th + at)];
+          const float w = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - m);
+          l = __builtin_fmaf(w, p.part_ml[2 * (z * th + at) + 1], l);
+          sum += w * *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+        }
+        f = l != 0.f ? 1.f / l : 0.f;
+      } else {
+        for (int z = 0; z < used; ++z) sum += *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+      }
+      *(cu32x2_t*)(p.o + (int64_t)(sp.tok0 + t) * p.o_st + (int64_t)h * p.o_sh + d) =
+          cu32x2_t{cpack(sum[0] * f, sum[1] * f), cpack(sum[2] * f, sum[3] * f)};
+    }
+  }
+}
+
+
+constexpr int64_t kMaxSeq = (int64_t)1 << 28;
+constexpr int kCUs = 256;  // MI355X compute units
+
+int block_shift(int32_t bs) {
+  for (int s = 4; s <= 8; ++s)
+    if (bs == 1 << s) return s;
+  return -1;
+}
+
+int validate(const chia_cache_attn_args* a) {
+  if (!a || !a->attn) return CHIA_ATTN_ERR_NULL;
+  if (a->struct_size != sizeof(chia_cache_attn_args) || a->reserved0 != 0) return CHIA_ATTN_ERR_STRUCT;
+  for (int i = 0; i < 8; ++i)
+    if (a->reserved[i] != 0) return CHIA_ATTN_ERR_STRUCT;
+  const chia_attn_args* t = a->attn;
+  if (t->struct_size != sizeof(chia_attn_args) || t->reserved0 != 0 || t->reserved[0] != 0 || t->reserved[1] != 0)
+    return CHIA_ATTN_ERR_STRUCT;
+  if (a->format > CHIA_ATTN_FP8_E5M2 || t->norm > CHIA_ATTN_NORM_RELU) return CHIA_ATTN_ERR_NORM;
+  if (t->head_dim != 64 && t->head_dim != 128) return CHIA_ATTN_ERR_HEAD_DIM;
+  const int shift = block_shift(a->block_size);
+  if (shift < 0 || t->batch < 1 || t->batch > (1 << 24) || t->heads < 1 || t->heads > (1 << 16) || t->kv_heads < 0 ||
+      (t->kv_heads > 0 && t->heads % t->kv_heads != 0) || t->seqlen < 1 || t->seqlen >= kMaxSeq || a->width < 1 ||
+      a->table_stride < 0 || a->width > (kMaxSeq >> shift) || a->num_blocks < 1 ||
+      a->num_blocks > (INT32_MAX >> shift) || a->queries < 0 || a->queries > kMaxSeq ||
+      a->queries * t->heads > ((int64_t)1 << 30) || a->max_query < 1 ||
+      (!t->cu_seqlens && a->queries != t->batch))
+    return CHIA_ATTN_ERR_SHAPE;
+  if (t->window < 0 || t->dilation < 1 || t->block < 0 || t->prefix < 0 || (t->dilation > 1 && t->prefix > 0))
+    return CHIA_ATTN_ERR_MASK;
+  if (!(t->scale > 0.f) || !std::isfinite(t->scale) || !(t->softcap >= 0.f) || !std::isfinite(t->softcap) ||
+      !std::isfinite(t->bias) || !std::isfinite(t->post_scale))
+    return CHIA_ATTN_ERR_SCALE;
+  return CHIA_ATTN_OK;
+}
+
+// The launch: which row tile, how many of them per (request, K/V head), and how
+// the steps of a tile's walk are split.
+struct Shape {
+  int tile;
+  int64_t tiles, parts, chunk;
+};
+
+Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
+  const chia_attn_args* t = a->attn;
+  const int64_t hkv = t->kv_heads > 0 ? t->kv_heads : t->heads, G = t->heads / hkv;
+  const int64_t most = !t->cu_seqlens ? 1 : a->max_query < a->queries ? a->max_query : a->queries;
+  const int64_t rows = G * (most < 1 ? 1 : most);
+  Shape s;
+  s.tile = rows <= 16 ? CACHE_ROWS16 : rows <= 32 ? CACHE_ROWS32 : CACHE_ROWS128;
+  const int R = kCacheRows[s.tile];
+  s.tiles = (rows + R - 1) / R;
+  // steps of the longest request's last tile
+  const int64_t S = t->seqlen < (a->width * a->block_size) ? t->seqlen : a->width * a->block_size;
+  const int64_t span = (R + G - 1) / G;
+  const int32_t i0 = (int32_t)(S - (span < most ? span : most));
+  const TileWalk w = cache_tile_walk(m, i0 < 0 ? 0 : i0, (int32_t)S - 1, (int32_t)S);
+  const int64_t steps = w.n > 0 ? w.n : 1;
+  const int64_t groups = t->batch * hkv * s.tiles;
+  // Enough workgroups for two rounds of three per CU, each with two steps or more per wavefront.
+  const int64_t want = (6 * kCUs + groups - 1) / groups;
+  const int64_t least = s.tile == CACHE_ROWS128 ? 16 : 8;
+  s.chunk = (steps + want - 1) / want;
+  if (s.chunk < least) s.chunk = least;
+  s.parts = (steps + s.chunk - 1) / s.chunk;
+  return s;
+}
+
+CacheMask mask_of(const chia_attn_args* t) {
+  CacheMask m;
+  // a reach past every length is none
+  m.causal = t->causal ? 1 : 0;
+  m.window = t->window < kMaxSeq ? t->window : 0;
+  m.dil = t->dilation < kMaxSeq ? t->dilation : (int32_t)kMaxSeq;
+  m.blk = t->block < kMaxSeq ? t->block : 0;
+  m.prefix = t->prefix < kMaxSeq ? t->prefix : (int32_t)kMaxSeq;
+  m.div_blk = make_udiv(m.blk > 0 ? m.blk : 1);
+  m.div_dil = make_udiv(m.dil);
+  return m;
+}
+
+template <int D, bool SOFTMAX>
+CacheAttnFn merge_of(int tile) {
+  return tile == CACHE_ROWS16 ? cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS16]>
+         : tile == CACHE_ROWS32 ? cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS32]>
+                                : cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS128]>;
+}
+
+CacheAttnFn merge_kernel(int head_dim, bool softmax, int tile) {
+  return head_dim == 64 ? (softmax ? merge_of<64, true>(tile) : merge_of<64, false>(tile))
+                        : (softmax ? merge_of<128, true>(tile) : merge_of<128, false>(tile));
+}
+
+int64_t workspace_of(const chia_cache_attn_args* a, const Shape& s) {
+  return s.parts > 1 ? s.parts * a->queries * a->attn->heads * (a->attn->head_dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
+}  // namespace
+}  // namespace chia
+
+using namespace chia;
+
+extern "C" int64_t chia_cache_attn_workspace_size(const chia_cache_attn_args* a) {
+  const int st = validate(a);
+  if (st != CHIA_ATTN_OK) return st;
+  return workspace_of(a, shape_of(a, mask_of(a->attn)));
+}
+
+extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
+  const int st = validate(a);
+  if (st != CHIA_ATTN_OK) return st;
+  if (a->queries == 0) return CHIA_ATTN_OK;
+  const chia_attn_args* t = a->attn;
+  if (!t->q || !t->k || !t->v || !t->o || !a->k_scale || !a->v_scale || !a->block_tables || !a->seq_lens)
+    return CHIA_ATTN_ERR_NULL;
+  for (const void* ptr : {t->q, t->k, t->v, (const void*)t->o, (const void*)a->workspace})
+    if ((uintptr_t)ptr & 15u) return CHIA_ATTN_ERR_ALIGN;
+  for (const void* ptr : {(const void*)a->k_scale, (const void*)a->v_scale, (const void*)a->block_tables,
+                          (const void*)a->seq_lens, (const void*)t->cu_seqlens, (const void*)t->head_scale,
+                          (const void*)t->alibi_slopes})
+    if ((uintptr_t)ptr & 3u) return CHIA_ATTN_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i)
+    if ((i > 0 && (t->q_stride[i] % 8 || t->o_stride[i] % 8)) || t->k_stride[i] % 16 || t->v_stride[i] % 16)
+      return CHIA_ATTN_ERR_ALIGN;
+  // a lane reaches the 16 tokens of a load with 32-bit offsets
+  for (const int64_t* sd : {t->k_stride, t->v_stride})
+    if (sd[2] < 0 || sd[2] >= ((int64_t)1 << 26)) return CHIA_ATTN_ERR_SHAPE;
+
+  CacheAttnParams p{};
+  p.mask = mask_of(t);
+  const Shape s = shape_of(a, p.mask);
+  const int64_t bytes = workspace_of(a, s);
+  if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes)) return CHIA_ATTN_ERR_WORKSPACE;
+  p.q = (const uint16_t*)t->q;
+  p.o = (uint16_t*)t->o;
+  p.k = (const uint8_t*)t->k;
+  p.v = (const uint8_t*)t->v;
+  p.ks = a->k_scale;
+  p.vs = a->v_scale;
+  p.q_sh = t->q_stride[1], p.q_st = t->q_stride[2];
+  p.o_sh = t->o_stride[1], p.o_st = t->o_stride[2];
+  p.k_sb = t->k_stride[0], p.k_sh = t->k_stride[1], p.k_st = t->k_stride[2];
+  p.v_sb = t->v_stride[0], p.v_sh = t->v_stride[1], p.v_st = t->v_stride[2];
+  p.ks_sb = a->k_scale_stride[0], p.ks_sh = a->k_scale_stride[1];
+  p.vs_sb = a->v_scale_stride[0], p.vs_sh = a->v_scale_stride[1];
+  p.table = a->block_tables;
+  p.table_stride = a->table_stride;
+  p.lens = a->seq_lens;
+  p.cu = t->cu_seqlens;
+  p.head_scale = t->head_scale;
+  p.alibi = t->alibi_slopes;
+  p.R = (int32_t)t->batch;
+  p.H = (int32_t)t->heads;
+  p.Hkv = t->kv_heads > 0 ? t->kv_heads : p.H;
+  p.G = p.H / p.Hkv;
+  p.T = (int32_t)a->queries;
+  p.width = (int32_t)a->width;
+  p.num_blocks = (int32_t)a->num_blocks;
+  p.bshift = block_shift(a->block_size);
+  p.tiles = (int32_t)s.tiles;
+  p.parts = (int32_t)s.parts;
+  p.chunk = (int32_t)s.chunk;
+  p.div_parts = make_udiv(p.parts);
+  p.div_tiles = make_udiv(p.tiles);
+  p.div_hkv = make_udiv(p.Hkv);
+  p.div_g = make_udiv(p.G);
+  p.scale = t->scale;
+  p.softcap = t->softcap;
+  p.bias = t->bias;
+  p.post_scale = t->post_scale;
+  p.part_o = (float*)a->workspace;
+  p.part_ml = bytes > 0 ? p.part_o + s.parts * a->queries * t->heads * t->head_dim : nullptr;
+  const int64_t units = t->batch * p.Hkv * s.tiles, wgs = units * s.parts;
+  if (wgs > INT32_MAX / 4) return CHIA_ATTN_ERR_SHAPE;
+
+  const int score = t->norm == CHIA_ATTN_NORM_SIGMOID ? CACHE_SIGMOID
+                    : t->norm == CHIA_ATTN_NORM_RELU  ? CACHE_RELU
+                    : t->alibi_slopes || t->softcap > 0.f ? CACHE_SOFTMAX_MOD : CACHE_SOFTMAX;
+  const CacheAttnFn fn = t->head_dim == 64 ? select_cache_kernel_d64((int)a->format, score, s.tile)
+                                           : select_cache_kernel_d128((int)a->format, score, s.tile);
+  if (!fn) return CHIA_ATTN_ERR_NORM;
+  void* kargs[] = {&p};
+  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)wgs), dim3(256), kargs, 0,
+                                   (hipStream_t)stream);
+  if (err == hipSuccess && s.parts > 1)
+    err = hipLaunchKernel(reinterpret_cast<const void*>(merge_kernel((int)t->head_dim, t->norm == CHIA_ATTN_NORM_SOFTMAX, s.tile)), dim3((unsigned)units), dim3(256), kargs, 0,
+                          (hipStream_t)stream);
+  if (err != hipSuccess) return (int)err;
+  err = hipGetLastError();
+  return err == hipSuccess ? CHIA_ATTN_OK : (int)err;
+}

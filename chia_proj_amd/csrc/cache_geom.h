@@ -1,0 +1,85 @@
+// cache_geom.h -- which keys of the paged cache a query sees, and how a row
+// tile's keys are walked and split; shared by the kernels, the launch code and
+// host checks.
+//
+// For one query at position i of a request with S tokens the mask of mask.h is
+//   visible(j) = j < S and (j < pre  or  (lo <= j < hi and (i - j) % dil == 0)).
+// A row tile holds queries at positions i0 .. i1 (times the query heads of one
+// K/V head).  Its keys are walked in steps of 32: the prefix's steps, then those
+// of the band that lie behind them.  The steps are split evenly enough: `parts`
+// workgroups take `chunk` steps each, chunk being the launch's, or more where a
+// request is longer than the launch was told.
+#pragma once
+#include "mask.h"
+
+namespace chia {
+
+constexpr int kStepKeys = 32;
+
+// A table's page number, or -1 for one outside the cache: such a page is not read.
+CHIA_HD int32_t cache_page(int32_t id, int32_t num_blocks) { return (uint32_t)id < (uint32_t)num_blocks ? id : -1; }
+
+// A slot, or -1 for one outside the cache: such a token is not written.
+CHIA_HD int32_t cache_slot(int32_t slot, int32_t num_slots) { return (uint32_t)slot < (uint32_t)num_slots ? slot : -1; }
+
+struct CacheMask {
+  int32_t causal, window, dil, blk, prefix;  // window, blk, prefix below 2^28; 0 = off
+  UDiv div_blk, div_dil;
+};
+
+struct RowKeys {
+  int32_t lo, hi, pre;  // lo <= j < hi (and the dilation), or j < pre
+};
+
+CHIA_HD RowKeys cache_row_keys(const CacheMask& m, int32_t i, int32_t S) {
+  if (i < 0) return {0, 0, 0};
+  int32_t lo = 0, hi = S;
+  if (m.causal) hi = imin32(hi, i + 1);
+  if (m.window > 0) {
+    lo = imax32(lo, i - m.window + 1);
+    if (!m.causal) hi = imin32(hi, i + m.window);
+  }
+  if (m.blk > 0) {
+    const int32_t b = udiv(i, m.div_blk) * m.blk;
+    lo = imax32(lo, b);
+    hi = imin32(hi, b + m.blk);
+  }
+  return {lo, hi, imin32(m.prefix, S)};
+}
+
+// The walk of a row tile: step s covers keys key_of(s) .. + 31.
+struct TileWalk {
+  int32_t n_pre, first, n;          // prefix steps, first band step, steps in all
+  int32_t full_lo, full_hi, full_pre;  // every row sees [full_lo, full_hi) and [0, full_pre) (dilation 1)
+};
+
+CHIA_HD TileWalk cache_tile_walk(const CacheMask& m, int32_t i0, int32_t i1, int32_t S) {
+  // lo and hi never fall with the position: the first row reaches lowest, the last highest.
+  const RowKeys a = cache_row_keys(m, imax32(i0, 0), S), b = cache_row_keys(m, i1, S);
+  TileWalk w;
+  const int32_t pre = b.pre;
+  w.n_pre = (pre + kStepKeys - 1) / kStepKeys;
+  w.first = imax32(w.n_pre, a.lo / kStepKeys);
+  w.n = w.n_pre + imax32(0, (b.hi + kStepKeys - 1) / kStepKeys - w.first);
+  if (i1 < 0) w.n_pre = w.n = 0;
+  w.full_lo = b.lo;
+  w.full_hi = i0 < 0 || m.dil > 1 ? 0 : a.hi;
+  w.full_pre = i0 < 0 ? 0 : pre;
+  return w;
+}
+
+CHIA_HD int32_t walk_key(const TileWalk& w, int32_t s) {
+  return kStepKeys * (s < w.n_pre ? s : w.first + (s - w.n_pre));
+}
+
+// Whether every row of the tile sees all of keys c .. c + n - 1.
+CHIA_HD bool walk_full(const TileWalk& w, int32_t c, int32_t n) {
+  return (c >= w.full_lo && c + n <= w.full_hi) || c + n <= w.full_pre;
+}
+
+// Steps of each part, of at most `parts`.
+CHIA_HD int32_t walk_chunk(int32_t steps, int32_t parts, int32_t chunk) {
+  return imax32(chunk, (steps + parts - 1) / parts);
+}
+
+}  // namespace chia

@@ -322,3 +322,78 @@ def call_fwd_fp8(q: Tensor, k: Tensor, v: Tensor, q_descale: float, k_descale: f
                                        params["head_scale"], params["alibi_slopes"],
                                        float(params["softcap"] or 0.0), float(params["bias"]),
                                        float(params["post_scale"]))
+
+
+# ---- serving over a paged 8-bit cache ------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::extend_block_tables", mutates_args=("block_tables",), device_types="cuda")
+def extend_block_tables(block_tables: Tensor, context_lens: Tensor, new_lens: Tensor, free_blocks: Tensor,
+                        free_count: Tensor, block_size: int, max_tokens: int
+                        ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    from .cache import extend_block_tables as impl
+
+    step = impl(block_tables, context_lens, new_lens, free_blocks, free_count, block_size=block_size,
+                max_tokens=max_tokens)
+    return tuple(t.clone() for t in step)  # an operator's results do not share memory
+
+
+@extend_block_tables.register_fake
+def _extend_block_tables_fake(block_tables, context_lens, new_lens, free_blocks, free_count, block_size, max_tokens):
+    R = block_tables.shape[0]
+    return tuple(block_tables.new_empty((n,)) for n in (max_tokens, max_tokens, R + 1, R, 1, 1))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::release_block_tables", mutates_args=("block_tables", "free_blocks"),
+                         device_types="cuda")
+def release_block_tables(block_tables: Tensor, context_lens: Tensor, finished: Tensor, free_blocks: Tensor,
+                         free_count: Tensor, block_size: int) -> Tensor:
+    from .cache import release_block_tables as impl
+
+    return impl(block_tables, context_lens, finished, free_blocks, free_count, block_size=block_size)
+
+
+@release_block_tables.register_fake
+def _release_block_tables_fake(block_tables, context_lens, finished, free_blocks, free_count, block_size):
+    return block_tables.new_empty((1,))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::write_cache", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
+                         device_types="cuda")
+def write_cache(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor,
+                slots: Tensor) -> None:
+    from .cache import write_cache as impl
+
+    impl(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+
+
+@write_cache.register_fake
+def _write_cache_fake(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::attention_cache", mutates_args=(), device_types="cuda")
+def attention_cache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor,
+                    block_tables: Tensor, seq_lens: Tensor, cu_seqlens: Optional[Tensor], max_query: Optional[int],
+                    max_seqlen: Optional[int], norm: str, causal: bool, window: int, dilation: int, block: int,
+                    prefix: int, scale: Optional[float], head_scale: Optional[Tensor], alibi_slopes: Optional[Tensor],
+                    softcap: float, bias: float, post_scale: float) -> Tensor:
+    from .cache import attention_cache as impl
+
+    return impl(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_seqlens, max_query=max_query,
+                max_seqlen=max_seqlen, **_params(norm, causal, window, dilation, block, prefix, scale, head_scale,
+                                                 alibi_slopes, softcap, bias, post_scale))
+
+
+@attention_cache.register_fake
+def _attention_cache_fake(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_seqlens, max_query,
+                          max_seqlen, norm, causal, window, dilation, block, prefix, scale, head_scale, alibi_slopes,
+                          softcap, bias, post_scale):
+    torch._check(q.dim() == 3, lambda: "q must be 3-D [T, H, D]")
+    return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+
+
+def call_cache_attn(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_seqlens, max_query, max_seqlen,
+                    params: dict) -> Tensor:
+    """torch.ops.chia_attn.attention_cache with attention_cache()'s keyword parameters."""
+    return torch.ops.chia_attn.attention_cache(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                                               cu_seqlens, max_query, max_seqlen, *_schema_args(params))

@@ -1,0 +1,696 @@
+"""GPU tests of the paged 8-bit cache against its float64 oracle (oracle/cache.py).
+
+Whole numbers, codes and scales have to be equal.  Attention outputs have the
+tolerance that their roundings give: every weight is rounded to bf16 (at most
+2^-8 relative; the softmax sum adds the rounded weights, so twice that), the
+scores are fp32 (the oracle's `slack`), the output is rounded to bf16 once.
+"""
+import pytest
+import torch
+
+import chia_proj_amd as lib
+from oracle import cache as oc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
+U = 2.0 ** -8
+
+
+def _say(msg):
+    print(msg, flush=True)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- block tables -----------------------------------------------------------------
+
+def _tables_case(R, width, bs, seed, spare=5, longest=None):
+    g = _gen(seed)
+    ctx = [int(x) for x in torch.randint(0, (longest or width * bs // 2) + 1, (R,), generator=g)]
+    new = [int(x) for x in torch.randint(0, width * bs // 2, (R,), generator=g)]
+    for r in range(0, R, 5):
+        new[r] = 0
+    for r in range(1, R, 7):
+        ctx[r] = 0
+    have = [-(-c // bs) for c in ctx]
+    want = sum(-(-(c + n) // bs) - h for c, n, h in zip(ctx, new, have))
+    pages = torch.randperm(sum(have) + want + spare, generator=g).tolist()
+    table = []
+    for h in have:
+        table.append([pages.pop() for _ in range(h)] + [-7] * (width - h))
+    return table, ctx, new, pages
+
+
+def _check_tables(table, ctx, new, free, count, bs, T):
+    want = oc.tables_ref(table, ctx, new, free, count, bs, T)
+    t = _i32(table).to(DEV)
+    args = [_i32(x).to(DEV) for x in (ctx, new, free)] + [_i32([count]).to(DEV)]
+    for _ in range(2):  # the same inputs again give the same
+        step = lib.extend_block_tables(t, *args, block_size=bs, max_tokens=T)
+        got = (t.tolist(), *(x.tolist() for x in step[:4]), int(step.free_count), int(step.missing))
+        for name, a, b in zip(("table", "slots", "positions", "cu", "lens", "left", "missing"), got, want):
+            assert a == b, name
+    assert args[2].tolist() == free and int(args[3]) == count
+    return step
+
+
+@pytest.mark.parametrize("R,width,bs", [(1, 1, 16), (1, 7, 256), (3, 5, 16), (64, 20, 32), (300, 9, 64), (1024, 4, 16),
+                                        (1025, 3, 16), (2500, 4, 32)])
+def test_tables(R, width, bs):
+    _say(f"[tables] {R} {width} {bs}")
+    table, ctx, new, free = _tables_case(R, width, bs, R + width)
+    T = sum(new)
+    _check_tables(table, ctx, new, free, len(free), bs, T + 3)
+    _check_tables(table, ctx, new, free, len(free), bs, T)
+
+
+def test_tables_that_do_not_suffice():
+    _say("[tables] shortage")
+    table, ctx, new, free = _tables_case(40, 12, 16, 3)
+    T = sum(new)
+    for count in (0, 1, 7, len(free) // 2):
+        _check_tables(table, ctx, new, free, count, 16, T)
+    _check_tables(table, ctx, new, free, len(free) + 9, 16, T)  # a count past the list's end
+    _check_tables(table, ctx, new, free, -4, 16, T)
+    _check_tables(table, ctx, new, free, len(free), 16, T // 2)  # fewer rows than tokens
+    _check_tables(table, ctx, new, free, len(free), 16, 0)
+    wide = [n + 300 for n in new]  # requests that outgrow the table's width
+    _check_tables(table, ctx, wide, list(range(5000)), 5000, 16, sum(wide))
+    _check_tables(table, ctx, [-n for n in new], free, len(free), 16, 4)
+    _check_tables([[-1, -1, -1], [-1, 4, -1]], [20, 5], [20, 9], [0, 1, 2], 3, 16, 29)  # pages begun that are not there
+    _check_tables([[3, -1], [-1, -1]], [16, 0], [0, 0], [], 0, 16, 2)
+
+
+def test_tables_row_stride_and_no_requests():
+    _say("[tables] strided")
+    table, ctx, new, free = _tables_case(6, 5, 16, 9)
+    big = torch.full((6, 11), -9, dtype=torch.int32, device=DEV)
+    big[:, 2:7] = _i32(table).to(DEV)
+    args = [_i32(x).to(DEV) for x in (ctx, new, free, [len(free)])]
+    step = lib.extend_block_tables(big[:, 2:7], *args, block_size=16, max_tokens=sum(new))
+    want = oc.tables_ref(table, ctx, new, free, len(free), 16, sum(new))
+    assert big[:, 2:7].tolist() == want[0] and step.slots.tolist() == want[1]
+    assert bool((big[:, :2] == -9).all()) and bool((big[:, 7:] == -9).all())
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    step = lib.extend_block_tables(big[:0], none, none, args[2], args[3], block_size=16, max_tokens=3)
+    assert step.slots.tolist() == [-1] * 3 and step.cu_seqlens.tolist() == [0] and int(step.free_count) == len(free)
+
+
+@pytest.mark.parametrize("R", [1, 9, 1100])
+def test_release(R):
+    _say(f"[release] {R}")
+    g = _gen(R)
+    table, ctx, _, free = _tables_case(R, 70, 16, R, longest=70 * 16)
+    done = (torch.rand(R, generator=g) < 0.5).tolist()
+    room = free + [-3] * 40000
+    want = list(free)
+    for r in range(R):
+        if done[r]:
+            want += [x for x in table[r][:-(-ctx[r] // 16)] if x >= 0]
+            table_r = [-1] * 70
+        else:
+            table_r = table[r]
+        table[r] = (table[r], table_r)
+    t = _i32([a for a, _ in table]).to(DEV)
+    f = _i32(room).to(DEV)
+    left = lib.release_block_tables(t, _i32(ctx).to(DEV), torch.tensor(done).to(DEV), f, _i32([len(free)]).to(DEV),
+                                    block_size=16)
+    assert int(left) == len(want) and f.tolist()[:len(want)] == want
+    assert bool((f[len(want):] == -3).all())
+    assert t.tolist() == [b for _, b in table]
+    # a stack without room for all of it takes what fits
+    t = _i32([a for a, _ in table]).to(DEV)
+    small = _i32((free + [-3] * 2)).to(DEV)
+    left = lib.release_block_tables(t, _i32(ctx).to(DEV), torch.tensor(done).to(DEV), small, _i32([len(free)]).to(DEV),
+                                    block_size=16)
+    assert small.tolist() == want[:len(free) + 2] + [-3] * (len(free) + 2 - len(want)) and int(left) == min(len(want), len(free) + 2)
+
+
+# ---- writing ----------------------------------------------------------------------
+
+def _filled(g, pages, H, bs, D, dtype, spread=2.0):
+    """Codes and power-of-two scales of pages that hold something, and garbage (NaN codes) in a few places."""
+    x = torch.randn(pages, H, bs, D, generator=g) * torch.exp(spread * torch.randn(pages, H, 1, 1, generator=g))
+    scale = torch.tensor([oc.need_scale(float(a), dtype) for a in x.abs().amax((2, 3)).reshape(-1)]).reshape(pages, H)
+    return (x / scale[:, :, None, None]).to(dtype), scale.float()
+
+
+def _same_codes(got, want, name):
+    got, want = got.cpu().float().double(), want
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), name
+    ok = torch.isnan(want) | (got == want)
+    assert bool(ok.all()), (name, int((~ok).sum()), got[~ok][:4], want[~ok][:4])
+
+
+def _check_write(k, v, kc, vc, ks, vs, slots):
+    want = [oc.write_ref(x, c, s, slots) for x, c, s in ((k, kc, ks), (v, vc, vs))]
+    dev = [x.to(DEV) for x in (k, v, kc, vc, ks, vs)]
+    lib.write_cache(*dev, _i32(slots).to(DEV))
+    torch.cuda.synchronize()
+    for name, got, (codes, scale), g_s in (("k", dev[2], want[0], dev[4]), ("v", dev[3], want[1], dev[5])):
+        assert torch.equal(g_s.cpu().double(), scale), name
+        _same_codes(got, codes, name)
+    return dev
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_write(dtype, D, bs):
+    """Runs that fill pages, begin and end inside them, single tokens, tokens without a slot."""
+    _say(f"[write] {dtype} {D} {bs}")
+    g = _gen(bs + D)
+    H, pages = 3, 9
+    kc, ks = _filled(g, pages, H, bs, D, dtype)
+    vc, vs = _filled(g, pages, H, bs, D, dtype)
+    slots = [4 * bs + i for i in range(bs // 2, bs)] + [bs * 7 + i for i in range(bs)] + [bs * 2 + i for i in range(5)]
+    slots += [-1, -1] + [0 * bs + bs - 1] + [pages * bs, 1 << 30] + [3 * bs + 1, 3 * bs + 2] + [5 * bs]
+    T = len(slots)
+    k = (torch.randn(T, H, D, generator=g) * torch.exp(2 * torch.randn(T, H, 1, generator=g))).to(torch.bfloat16)
+    v = torch.randn(T, H, D, generator=g).to(torch.bfloat16) * 0.01
+    _check_write(k, v, kc, vc, ks, vs, slots)
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+def test_write_values_at_the_edges(dtype):
+    """Zeros, the smallest and largest bf16 numbers, values next to a scale's border, infinities and NaN."""
+    _say(f"[write] edges {dtype}")
+    g = _gen(4)
+    H, D, bs, pages = 2, 64, 16, 12
+    kc, ks = _filled(g, pages, H, bs, D, dtype)
+    T = pages
+    k = torch.randn(T, H, D, generator=g).to(torch.bfloat16)
+    top = oc.TOP[dtype]
+    k[0] = 0
+    k[1] = 0
+    k[1, :, 5] = 9.2e-41  # a subnormal
+    k[2, :, 3] = 3.38e38
+    k[3] = k[3] * 1e-30
+    k[4, :, 7] = float("inf")
+    k[4, :, 8] = float("-inf")
+    k[5, 0] = float("nan")
+    k[6] = 0
+    k[6, :, 0] = top * 0.125  # exactly a power of two times the largest value
+    k[7, :, :] = k[6]
+    k[7, :, 1] = float(torch.tensor(top * 0.125, dtype=torch.bfloat16).view(torch.int16).add(1).view(torch.bfloat16))
+    k[8] = float("inf")
+    k[9, :, ::2] = -0.0
+    begun = [p * bs + (3 if p % 2 else 0) for p in range(pages)]
+    _check_write(k, -k, kc, kc.clone(), ks, ks.clone(), begun)
+    _check_write(k, -k, kc, kc.clone(), ks, ks.clone(), [p * bs for p in range(pages)])
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+def test_write_keeps_old_codes_and_scales(dtype):
+    """A page that began keeps its scale where that is more, whatever number it is; kept codes follow one that grows."""
+    _say(f"[write] kept {dtype}")
+    g = _gen(6)
+    H, D, bs, pages = 2, 128, 32, 6
+    kc, ks = _filled(g, pages, H, bs, D, dtype)
+    ks = ks * torch.tensor([1.0, 1.3, 0.7, 1.0, 1.0, 1.0])[:, None]  # pages somebody else rounded
+    k = torch.randn(pages, H, D, generator=g).to(torch.bfloat16)
+    k[0], k[1], k[2], k[3], k[4] = k[0] * 1e4, k[1] * 1e-4, k[2] * 1e-4, k[3] * 1e9, k[4] * 1e-9
+    _check_write(k, k, kc, kc.clone(), ks, ks.clone(), [p * bs + bs - 1 - p for p in range(pages)])
+
+
+def test_write_many_tokens_in_windows():
+    """Enough tokens that a team looks for runs in a window of several, contiguous and one by one."""
+    _say("[write] windows")
+    g = _gen(8)
+    H, D, bs = 16, 64, 16
+    pages = 700
+    kc, ks = _filled(g, pages, H, bs, D, E4)
+    order = torch.randperm(pages, generator=g).tolist()
+    slots = [p * bs + i for p in order[:500] for i in range(bs)][3:]
+    slots += [p * bs + int(torch.randint(0, bs, (1,), generator=g)) for p in order[500:]]
+    k = torch.randn(len(slots), H, D, generator=g).to(torch.bfloat16)
+    assert 2 * H * len(slots) > 65536
+    _check_write(k, k * 3, kc, kc.clone(), ks, ks.clone(), slots)
+
+
+def test_write_strided_tensors():
+    """K and V as slices of one projection, caches of several layers interleaved, tokens before heads."""
+    _say("[write] strides")
+    g = _gen(10)
+    T, H, D, bs, pages = 37, 4, 64, 16, 5
+    qkv = torch.randn(T, 3 * H, D, generator=g).to(torch.bfloat16)
+    k, v = qkv[:, H:2 * H], qkv[:, 2 * H:]
+    c, s = _filled(g, pages, 2 * H, bs, D, E4)
+    slots = list(range(5, 5 + T))
+    want = [oc.write_ref(x, c[:, o:o + H], s[:, o:o + H], slots) for x, o in ((k, 0), (v, H))]
+    dev, cd, sd = qkv.to(DEV), c.to(DEV), s.to(DEV)
+    for layout in range(2):
+        cc = cd.clone() if layout == 0 else cd.clone().transpose(1, 2).contiguous().transpose(1, 2)
+        ss = sd.clone() if layout == 0 else sd.clone().t().contiguous().t()
+        lib.write_cache(dev[:, H:2 * H], dev[:, 2 * H:], cc[:, :H], cc[:, H:], ss[:, :H], ss[:, H:], _i32(slots).to(DEV))
+        for o, (codes, scale) in zip((0, H), want):
+            _same_codes(cc[:, o:o + H], codes, layout)
+            assert torch.equal(ss[:, o:o + H].cpu().double(), scale)
+
+
+# ---- attention --------------------------------------------------------------------
+
+class Case:
+    """Requests of the given lengths over a shuffled cache; what no query may see is poisoned."""
+
+    def __init__(self, lens, n=1, H=4, Hkv=2, D=64, bs=16, dtype=E4, seed=0, width=None, spread=0.3, poison=True):
+        g = _gen(seed + 1)
+        self.lens, R = list(lens), len(lens)
+        self.n = [n] * R if isinstance(n, int) else list(n)
+        self.bs, self.dtype = bs, dtype
+        width = width or max(1, max(-(-x // bs) for x in lens))
+        pages = sum(-(-x // bs) for x in lens) + 2
+        perm = torch.randperm(pages, generator=g).tolist()
+        self.table = torch.full((R, width), -1, dtype=torch.int32)
+        for r, x in enumerate(lens):
+            for c in range(-(-x // bs)):
+                self.table[r, c] = perm.pop()
+        k = torch.randn(pages, Hkv, bs, D, generator=g) * torch.exp(spread * torch.randn(pages, Hkv, 1, 1, generator=g))
+        v = torch.randn(pages, Hkv, bs, D, generator=g) * torch.exp(spread * torch.randn(pages, Hkv, 1, 1, generator=g))
+        scales = [torch.tensor([oc.need_scale(float(a), dtype) for a in x.abs().amax((2, 3)).reshape(-1)]).reshape(pages, Hkv).float()
+                  for x in (k, v)]
+        self.ks, self.vs = scales
+        self.kc, self.vc = ((x / s[:, :, None, None]).to(dtype) for x, s in zip((k, v), scales))
+        if poison:  # the rest of every last page, and pages nobody has
+            bad = 0x7F if dtype == E4 else 0x7D
+            for c in (self.kc, self.vc):
+                u = c.view(torch.uint8)
+                for r, x in enumerate(lens):
+                    if x % bs:
+                        u[self.table[r, x // bs].long(), :, x % bs:] = bad
+                for p in perm:
+                    u[p] = bad
+            for s in (self.ks, self.vs):
+                for p in perm:
+                    s[p] = float("nan")
+        self.cu = [0]
+        for m in self.n:
+            self.cu.append(self.cu[-1] + m)
+        self.q = torch.randn(self.cu[-1], H, D, generator=g).to(torch.bfloat16)
+
+    def device(self):
+        return [x.to(DEV) for x in (self.q, self.kc, self.vc, self.ks, self.vs, self.table, _i32(self.lens))]
+
+    def call(self, dev=None, **kw):
+        dev = dev or self.device()
+        cu = None if all(m == 1 for m in self.n) and not kw.pop("force_cu", False) else _i32(self.cu).to(DEV)
+        return lib.attention_cache(*dev, cu, **kw)
+
+    def check(self, o=None, hints=None, **kw):
+        if o is None:
+            o = self.call(**(hints if hints is not None else dict(max_query=max(self.n), max_seqlen=max(1, max(self.lens)))),
+                          **kw)
+        want, size, slack = oc.attend_ref(self.q, self.kc, self.vc, self.ks, self.vs, self.table, self.lens, self.cu, **kw)
+        rows = ~torch.isnan(want).all(-1).all(-1) | True
+        got = o.double().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN"
+        f = 2 if kw.get("norm", "softmax") == "softmax" else 1
+        bound = (f * U * (1 + U) * size + slack) * (1 + U) + U * want.abs() + 1e-37
+        err = (got - want).abs()
+        worst = float(torch.nan_to_num(err / bound).max()) if err.numel() else 0.0
+        assert worst <= 1.0, (worst, float(torch.nan_to_num(err).max()))
+        return o, rows
+
+
+LENS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 200, 513]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [E4, E5])
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (8, 8), (8, 2), (12, 4), (32, 2), (17, 1), (32, 1), (40, 1)])
+def test_decode(D, dtype, H, Hkv):
+    _say(f"[decode] {D} {dtype} {H}/{Hkv}")
+    Case(LENS, H=H, Hkv=Hkv, D=D, dtype=dtype, bs=32, seed=H).check()
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3])
+def test_page_sizes(bs, n):
+    _say(f"[pages] {bs} {n}")
+    Case([x + n for x in LENS], n=n, H=8, Hkv=4, D=128, bs=bs, seed=bs).check()
+
+
+VARIANTS = [dict(), dict(causal=False), dict(window=1), dict(window=40), dict(window=129, causal=False), dict(block=48),
+            dict(block=50, causal=False), dict(dilation=2), dict(dilation=3, window=70), dict(dilation=5, causal=False),
+            dict(prefix=20, window=16), dict(prefix=70, block=64), dict(prefix=600), dict(softcap=2.0),
+            dict(softcap=50.0, window=100), dict(alibi_slopes=[0.5, 0.25, 0.125, 0.0625]),
+            dict(alibi_slopes=[0.5, 0.25, 0.125, 0.0625], softcap=5.0, causal=False), dict(head_scale=[0.5, 1.0, 2.0, 4.0]),
+            dict(scale=0.5), dict(norm="sigmoid", bias=-3.0), dict(norm="sigmoid", causal=False, post_scale=0.25, window=33),
+            dict(norm="sigmoid", alibi_slopes=[0.1, 0.2, 0.3, 0.4], softcap=4.0), dict(norm="relu"),
+            dict(norm="relu", post_scale=0.01, prefix=9, window=5), dict(norm="relu", softcap=3.0, head_scale=[1., 2., 3., 4.])]
+
+
+@pytest.mark.parametrize("n", [1, [1, 3, 0, 7, 5, 2, 4], [60, 17, 0, 1, 33, 90, 64]])
+@pytest.mark.parametrize("kw", VARIANTS, ids=lambda kw: "-".join(f"{k}" for k in kw) or "plain")
+def test_variants(kw, n):
+    """Every mask, score modifier and normaliser, for single tokens, a few and many per request."""
+    _say(f"[variants] {kw} {n}")
+    lens = [1, 40, 64, 100, 33, 300, 517]
+    if not isinstance(n, int):
+        lens = [max(a, b) for a, b in zip(lens, n)]
+    for D, dtype, bs in ((64, E4, 16), (128, E5, 64)):
+        Case(lens, n=n, D=D, dtype=dtype, bs=bs, seed=3).check(**kw)
+
+
+@pytest.mark.parametrize("n", [1, 4, 70])
+@pytest.mark.parametrize("norm", ["softmax", "sigmoid"])
+def test_keys_split_over_workgroups(n, norm):
+    """Few rows and many keys: the keys are split and joined; the hints may be wrong in both directions."""
+    _say(f"[split] {n} {norm}")
+    kw = dict(norm=norm, bias=-6.0 if norm == "sigmoid" else 0.0)
+    c = Case([5003, 700, 64 + n], n=n, H=8, Hkv=2, D=128, bs=64, seed=n)
+    a, _ = c.check(**kw)
+    c.check(hints=dict(), **kw)
+    c.check(hints=dict(max_query=1, max_seqlen=33), **kw)
+    c.check(hints=dict(max_query=1 << 20, max_seqlen=1 << 27), **kw)
+    assert torch.equal(a, c.call(max_query=n, max_seqlen=5003, **kw))  # the same launch gives the same bits
+
+
+def test_long_request_in_small_pages():
+    """More pages than one look at the table holds (64), in each wavefront's share too."""
+    _say("[long]")
+    Case([40003], H=2, Hkv=1, D=64, bs=16, seed=5).check()
+    Case([9001], H=2, Hkv=1, D=64, bs=16, seed=5).check(hints=dict(max_seqlen=100))
+    Case([9001], H=2, Hkv=1, D=64, bs=16, seed=5).check(prefix=4000, window=300)
+
+
+def test_more_queries_than_tokens():
+    """Positions before the first token see nothing."""
+    _say("[short]")
+    for kw in (dict(), dict(causal=False), dict(prefix=3), dict(norm="sigmoid")):
+        Case([2, 0, 5], n=[6, 3, 5], seed=7).check(**kw)
+
+
+def test_pages_outside_the_cache():
+    """Table entries that name no page hide their tokens, in the middle and whole requests."""
+    _say("[bad pages]")
+    for n in (1, 5):
+        c = Case([300, 100, 64, 20], n=n, bs=16, seed=9)
+        c.table[0, 3], c.table[0, 7], c.table[1, 0] = -1, 1 << 30, c.kc.shape[0]
+        c.table[2, :] = -5
+        c.table[3, 1] = -(1 << 31)
+        o, _ = c.check()
+        assert float(o[c.cu[2]:c.cu[3]].abs().max()) == 0.0
+        c.check(norm="relu", window=50)
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_numbers_that_are_none_stay_where_they_are(dtype, n):
+    """NaN in keys and values that a query does not see does not reach it, and reaches it where it does."""
+    _say(f"[nan] {dtype} {n}")
+    bad = 0x7F if dtype == E4 else 0x7E
+    c = Case([200, 90], n=n, bs=16, dtype=dtype, D=128, seed=11)
+    for pos in (20, 199, 199 - n // 2):  # outside the window; seen by some of the queries
+        p = c.table[0, pos // 16].long()
+        c.vc.view(torch.uint8)[p, :, pos % 16, ::3] = bad
+        c.kc.view(torch.uint8)[p, 1, pos % 16, 0] = bad
+    p = c.table[1, 1].long()  # a whole page, its scale among it
+    c.vc.view(torch.uint8)[p] = bad
+    c.ks[p], c.vs[p] = float("nan"), float("inf")
+    want, _, _ = oc.attend_ref(c.q, c.kc, c.vc, c.ks, c.vs, c.table, c.lens, c.cu, window=48)
+    got = c.call(max_query=n, max_seqlen=200, window=48).double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = ~torch.isnan(want)
+    assert float((got - want)[fine].abs().max()) < 0.05 * float(want[fine].abs().max())
+
+
+def test_infinities_of_e5m2():
+    _say("[inf]")
+    c = Case([70], n=3, bs=16, dtype=E5, seed=13)
+    p = c.table[0, 4].long()
+    c.vc.view(torch.uint8)[p, 0, 4, 0] = 0x7C  # position 68: the last two of three queries see it
+    c.vc.view(torch.uint8)[p, 1, 5, 1] = 0xFC  # position 69: the last does
+    got = c.call(max_query=3, max_seqlen=70).float().cpu()
+    assert [float(got[t, 0, 0]) for t in (1, 2)] == [float("inf")] * 2 and float(got[2, 2, 1]) == float("-inf")
+    got[1:, :2, 0] = 0
+    got[2, 2:, 1] = 0
+    assert bool(torch.isfinite(got).all())
+
+
+def test_scales_that_are_no_powers_of_two():
+    _say("[scales]")
+    for n in (1, 40):
+        for norm in ("softmax", "sigmoid", "relu"):
+            c = Case([200, 77], n=n, bs=32, D=128, seed=15)
+            c.ks *= 1.37
+            c.vs *= torch.linspace(0.6, 1.9, c.vs.numel()).reshape(c.vs.shape)
+            c.check(norm=norm)
+
+
+def test_sharp_and_flat_scores():
+    """Scores that rise along the keys, so the running maximum moves often, and by far."""
+    _say("[sharp]")
+    for n in (1, 33):
+        c = Case([900], n=n, H=4, Hkv=2, D=64, bs=64, seed=17, spread=0.0)
+        c.ks *= torch.exp2(torch.arange(c.ks.shape[0]) % 7).float()[:, None]
+        c.check(scale=1.0)
+        c.check(scale=1e-4)
+        c.check(alibi_slopes=[3.0, 1.0, 0.5, 0.1])
+        c.check(alibi_slopes=[-3.0, -1.0, -0.5, -0.1])
+
+
+def test_layouts_and_out():
+    """Interleaved layers, tokens before heads, q as a slice of a projection, a strided `out` with rows behind the last."""
+    _say("[layouts]")
+    c = Case([100, 37, 64], n=[2, 1, 4], bs=16, D=64, seed=19)
+    base, _ = c.check()
+    q, kc, vc, ks, vs, table, lens = c.device()
+    both = torch.stack([kc.view(torch.uint8), vc.view(torch.uint8)], 1).view(c.dtype)
+    wide = torch.zeros(q.shape[0] + 5, 3, *q.shape[1:], dtype=torch.bfloat16, device=DEV)
+    wide[:-5, 1] = q
+    tokens_first = kc.transpose(1, 2).contiguous().transpose(1, 2)
+    strided_table = torch.full((3, 20), 1 << 20, dtype=torch.int32, device=DEV)
+    strided_table[:, 3:3 + table.shape[1]] = table
+    tb = strided_table[:, 3:3 + table.shape[1]]
+    out = torch.full((q.shape[0] + 5, 2, *q.shape[1:]), 7.0, dtype=torch.bfloat16, device=DEV)
+    cu = _i32(c.cu).to(DEV)
+    for kk, sk in ((both[:, 0], ks), (tokens_first, ks.t().contiguous().t())):
+        got = lib.attention_cache(wide[:, 1], kk, both[:, 1], sk, vs, tb, lens, cu, max_query=4, max_seqlen=100,
+                                  out=out[:, 0])
+        assert got.data_ptr() == out.data_ptr()
+        assert torch.equal(got[:-5], base)
+    assert bool((out[-5:] == 7).all()) and bool((out[:, 1] == 7).all())
+    odd = torch.empty(q.numel() + 3, dtype=torch.bfloat16, device=DEV)[3:].view(q.shape).copy_(q)  # not 16-byte aligned
+    assert torch.equal(lib.attention_cache(odd, kc, vc, ks, vs, table, lens, cu, max_query=4, max_seqlen=100), base)
+
+
+def test_one_table_row_for_all_requests():
+    """Requests that share their pages: an expanded table."""
+    _say("[shared]")
+    c = Case([200], n=1, bs=32, seed=21)
+    q = torch.randn(5, 4, 64, generator=_gen(2)).to(torch.bfloat16)
+    _, kc, vc, ks, vs, table, _ = c.device()
+    lens = [200, 10, 64, 0, 133]
+    got = lib.attention_cache(q.to(DEV), kc, vc, ks, vs, table.expand(5, -1), _i32(lens).to(DEV))
+    c.q, c.lens, c.n, c.cu, c.table = q, lens, [1] * 5, list(range(6)), c.table.expand(5, -1)
+    c.check(got)
+
+
+def test_offsets_past_32_bits():
+    """Pages more than 2^32 bytes from the cache's start."""
+    _say("[far]")
+    c = Case([150, 40], n=2, bs=64, D=128, H=4, Hkv=2, seed=23, poison=False)
+    pages = c.kc.shape[0]
+    store = torch.zeros((5 << 30) + (1 << 20), dtype=torch.uint8, device=DEV)
+    block = 1 << 30  # bytes from one page to the next
+    views = []
+    for i, x in enumerate((c.kc, c.vc)):
+        t = torch.as_strided(store.view(c.dtype), x.shape, (block, 64 * 128, 128, 1), i * 2 * 64 * 128)
+        t.view(torch.uint8).copy_(x.to(DEV).view(torch.uint8))
+        views.append(t)
+    assert (pages - 1) * block > 1 << 32
+    dev = c.device()
+    dev[1], dev[2] = views
+    o, _ = c.check(c.call(dev, max_query=2, max_seqlen=150))
+    slots = [(pages - 1) * 64 + 63]
+    k = torch.randn(1, 2, 128, generator=_gen(1)).to(torch.bfloat16)
+    want = oc.write_ref(k, c.kc, c.ks, slots)
+    lib.write_cache(k.to(DEV), k.to(DEV), views[0], views[1], dev[3], dev[4], _i32(slots).to(DEV))
+    _same_codes(views[0], want[0], "far write")
+
+
+# ---- together ---------------------------------------------------------------------
+
+def _serve(steps, H, Hkv, D, bs, dtype, R, pages, width, seed, use_graph=False):
+    """Prompts, then single tokens, through all three operators; after each step the output is
+    checked against attention over the cache as the oracle has written it."""
+    g = _gen(seed)
+    kc = torch.full((pages, Hkv, bs, D), float("nan")).to(dtype)  # memory as it comes
+    vc, ks, vs = kc.clone(), torch.full((pages, Hkv), float("nan")), torch.full((pages, Hkv), float("nan"))
+    d = [x.to(DEV) for x in (kc, vc, ks, vs)]
+    table = torch.full((R, width), -1, dtype=torch.int32, device=DEV)
+    t_ref = table.tolist()
+    free = torch.randperm(pages, generator=g).tolist()
+    free_d, count, lens = _i32(free).to(DEV), _i32([pages]).to(DEV), _i32([0] * R).to(DEV)
+    left, l_ref = pages, [0] * R
+    for new in steps:
+        T = sum(new) + 2
+        q, k, v = (torch.randn(T, h, D, generator=g).to(torch.bfloat16) for h in (H, Hkv, Hkv))
+        step = lib.extend_block_tables(table, lens, _i32(new).to(DEV), free_d, count, block_size=bs, max_tokens=T)
+        lib.write_cache(k.to(DEV), v.to(DEV), *d, step.slots)
+        out = torch.full((T, H, D), 5.0, dtype=torch.bfloat16, device=DEV)
+        lib.attention_cache(q.to(DEV), *d, table, step.seq_lens, step.cu_seqlens, max_query=max(new), out=out)
+        count, lens = step.free_count, step.seq_lens
+        t_ref, slots, _, cu, l_ref, left, missing = oc.tables_ref(t_ref, l_ref, new, free, left, bs, T)
+        assert (table.tolist(), step.slots.tolist(), int(count), int(step.missing)) == (t_ref, slots, left, missing)
+        assert missing == 0
+        kc64, ks64 = oc.write_ref(k, kc, ks, slots)
+        vc64, vs64 = oc.write_ref(v, vc, vs, slots)
+        kc, ks, vc, vs = kc64.to(dtype), ks64.float(), vc64.to(dtype), vs64.float()
+        _same_codes(d[0], kc64, "k")
+        want, size, slack = oc.attend_ref(q[:cu[-1]], kc, vc, ks, vs, _i32(t_ref), l_ref, cu)
+        err = (out[:cu[-1]].double().cpu() - want).abs()
+        assert bool((err <= (2 * U * (1 + U) * size + slack) * (1 + U) + U * want.abs()).all())
+        assert bool((out[cu[-1]:] == 5).all())
+    return table, lens, free_d, count
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+def test_serving(dtype):
+    _say(f"[serve] {dtype}")
+    steps = [[33, 0, 7, 50], [1, 1, 1, 1], [1, 16, 1, 1], [3, 0, 1, 2], [1, 1, 1, 1], [0, 0, 0, 20]]
+    table, lens, free, count = _serve(steps, 8, 2, 64, 16, dtype, 4, 40, 12, 1)
+    before = int(count)
+    held = [sum(x >= 0 for x in row) for row in table.tolist()]
+    left = lib.release_block_tables(table, lens, torch.tensor([False, True, False, True]).to(DEV), free, count, block_size=16)
+    assert int(left) == before + held[1] + held[3]
+    assert sorted(free.tolist()[:int(left)] + [x for r in (0, 2) for x in table[r].tolist() if x >= 0]) == list(range(40))
+
+
+def test_step_in_a_graph():
+    """One decoding step captured; replays follow what is copied into its inputs, with eager work between."""
+    _say("[graph]")
+    c = Case([300, 17, 64, 129], n=1, H=8, Hkv=2, D=128, bs=16, seed=31, width=25)
+    q, kc, vc, ks, vs, table, lens = c.device()
+    pages = kc.shape[0]
+    free, count = _i32([pages - 1, pages - 2]).to(DEV), _i32([0]).to(DEV)
+    new = _i32([1] * 4).to(DEV)
+    room = kc.shape[0]
+    spare = [int(x) for x in range(room)]
+    used = set(c.table[c.table >= 0].tolist())
+    free = _i32([x for x in spare if x not in used] * 1).to(DEV)
+    count = _i32([free.numel()]).to(DEV)
+    k, v = (torch.randn(4, 2, 128, generator=_gen(s)).to(torch.bfloat16).to(DEV) for s in (1, 2))
+    out = torch.empty_like(q)
+
+    def step():
+        s = lib.extend_block_tables(table, lens, new, free, count, block_size=16, max_tokens=4)
+        lib.write_cache(k, v, kc, vc, ks, vs, s.slots)
+        lib.attention_cache(q, kc, vc, ks, vs, table, s.seq_lens, max_seqlen=400, out=out)
+        return s
+
+    saved = [x.clone() for x in (kc, vc, ks, vs, table)]
+
+    def restore():
+        for x, y in zip((kc, vc, ks, vs, table), saved):
+            x.view(torch.uint8).copy_(y.view(torch.uint8)) if x.dtype == c.dtype else x.copy_(y)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    restore()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = step()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=_gen(40 + i)).to(torch.bfloat16))
+        k.copy_(torch.randn(k.shape, generator=_gen(50 + i)).to(torch.bfloat16) * (1 + i))
+        restore()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, codes, slots = out.clone(), kc.clone(), s.slots.clone()
+        restore()
+        out.zero_()
+        e = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out) and torch.equal(codes.view(torch.uint8), kc.view(torch.uint8))
+        assert torch.equal(slots, e.slots) and int(e.missing) == int(s.missing)
+
+
+def test_another_stream_and_two_calls_at_once():
+    _say("[streams]")
+    a, b = Case([3000], H=4, Hkv=1, D=64, bs=32, seed=33), Case([2500, 40], n=3, H=8, Hkv=2, D=128, bs=16, seed=34)
+    ad, bd = a.device(), b.device()
+    want = a.call(ad, max_seqlen=3000), b.call(bd, max_query=3, max_seqlen=2500)
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s):
+            x = a.call(ad, max_seqlen=3000)
+        with torch.cuda.stream(t):
+            y = b.call(bd, max_query=3, max_seqlen=2500)
+        torch.cuda.synchronize()
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
+def test_compiled_step():
+    """torch.compile keeps each operator as one node; the mutated tensors are the caller's."""
+    _say("[compile]")
+    c = Case([40, 17], n=1, H=4, Hkv=2, D=64, bs=16, seed=35, width=6)
+
+    def step(q, k, v, kc, vc, ks, vs, table, lens, new, free, count):
+        s = lib.extend_block_tables(table, lens, new, free, count, block_size=16, max_tokens=2)
+        lib.write_cache(k, v, kc, vc, ks, vs, s.slots)
+        return lib.attention_cache(q, kc, vc, ks, vs, table, s.seq_lens, max_seqlen=64) * 2, s.slots
+
+    k = torch.randn(2, 2, 64, generator=_gen(3)).to(torch.bfloat16).to(DEV)
+    results = []
+    for fn in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        q, kc, vc, ks, vs, table, lens = c.device()
+        o, slots = fn(q, k, -k, kc, vc, ks, vs, table, lens, _i32([1, 1]).to(DEV), _i32([0, 1]).to(DEV), _i32([2]).to(DEV))
+        results.append((o, slots, kc.view(torch.uint8), table))
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
+def test_gpu_refusals():
+    c = Case([40, 17], n=1, seed=37)
+    q, kc, vc, ks, vs, table, lens = c.device()
+    call = lib.attention_cache
+    with pytest.raises(ValueError, match="one query"):
+        call(q[:1], kc, vc, ks, vs, table, lens)
+    with pytest.raises(TypeError, match="bfloat16"):
+        call(q.float(), kc, vc, ks, vs, table, lens)
+    with pytest.raises(ValueError, match="dividing"):
+        call(q[:, :3], kc, vc, ks, vs, table, lens)
+    with pytest.raises(TypeError, match="seq_lens"):
+        call(q, kc, vc, ks, vs, table, lens.long())
+    with pytest.raises(ValueError, match="seq_lens"):
+        call(q, kc, vc, ks, vs, table, lens[:1])
+    with pytest.raises(ValueError, match="contiguous"):
+        call(q, kc, vc, ks, vs, table, lens.repeat_interleave(2)[::2])
+    with pytest.raises(TypeError, match="k_scale"):
+        call(q, kc, vc, ks.double(), vs, table, lens)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        call(q, kc, vc, ks, vs, table, lens, lens)
+    with pytest.raises(ValueError, match="is on cpu"):
+        call(q.cpu(), kc, vc, ks, vs, table, lens)
+    with pytest.raises(ValueError, match="prefix"):
+        call(q, kc, vc, ks, vs, table, lens, prefix=2, dilation=2)
+    with pytest.raises(ValueError, match="max_query"):
+        call(q, kc, vc, ks, vs, table, lens, max_query=0)
+    with pytest.raises(ValueError, match="out must"):
+        call(q, kc, vc, ks, vs, table, lens, out=torch.empty_like(q)[:, :2])
+    with pytest.raises(ValueError, match="free_count"):
+        lib.extend_block_tables(table, lens, lens, lens, lens, block_size=16, max_tokens=4)
+    with pytest.raises(ValueError, match="max_tokens"):
+        lib.extend_block_tables(table, lens, lens, lens, lens[:1], block_size=16, max_tokens=-1)
+    with pytest.raises(TypeError, match="finished"):
+        lib.release_block_tables(table, lens, lens, lens, lens[:1], block_size=16)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="T, H_kv, D"):
+        lib.write_cache(k[:1], k, kc, vc, ks, vs, lens)
+    with pytest.raises(TypeError, match="slots"):
+        lib.write_cache(k, k, kc, vc, ks, vs, lens.long())
+    assert call(q[:0], kc, vc, ks, vs, table[:0], lens[:0]).shape == (0, 4, 64)
