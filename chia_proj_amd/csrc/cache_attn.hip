@@ -9,46 +9,78 @@ namespace chia {
 namespace {
 
 // Joins the parts of rows whose keys were split: o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z.
-// 32 (D = 128) or 16 lanes to a row, float4 each.
-template <int D, bool SOFTMAX, int ROWS>
+// 32 (D = 128) or 16 lanes to a row, float4 each; ZG groups of them share a row's
+// parts and meet in LDS, so that a few rows of many parts are not one lane's walk.
+template <int D, bool SOFTMAX, int ROWS, int ZG>
 __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnParams p) {
-  constexpr int LPR = D / 4, PER = 256 / LPR;  // lanes per row, rows at a time
-  const int rh = udiv((int)blockIdx.x, p.div_tiles), rt0 = (int)blockIdx.x - rh * p.tiles;
+  constexpr int LPR = D / 4, SLOTS = 256 / LPR, RPW = SLOTS / ZG, SUBS = ROWS / RPW;
+  __shared__ f32x4_t sum_s[ZG > 1 ? 256 : 1];
+  __shared__ float ml_s[SLOTS][2];
+  const int u = (int)blockIdx.x / SUBS, sub = (int)blockIdx.x % SUBS;
+  const int rh = udiv(u, p.div_tiles), rt0 = u - rh * p.tiles;
   const int r = udiv(rh, p.div_hkv), hk = rh - r * p.Hkv;
   const CacheSpan sp = cache_span(p, r);
   const int n_rows = sp.n * p.G;
-  for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
+  const int slot = (int)threadIdx.x / LPR, d = 4 * ((int)threadIdx.x % LPR), zi = slot % ZG;
+  const int64_t th = (int64_t)p.T * p.H;
+  for (int rt = rt0; rt * ROWS + sub * RPW < n_rows; rt += p.tiles) {
     const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
     const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
     const int used = (tw.n + chunk - 1) / chunk;
     if (used <= 1) continue;
-    for (int i = (int)threadIdx.x / LPR; i < ROWS; i += PER) {
-      const int row = rt * ROWS + i;
-      if (row >= n_rows) break;
-      const int t = udiv(row, p.div_g), h = hk * p.G + row - t * p.G;
-      const int64_t th = (int64_t)p.T * p.H, at = (int64_t)(sp.tok0 + t) * p.H + h;
-      const int d = 4 * ((int)threadIdx.x % LPR);
-      float f = p.post_scale;
-      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    const int row = rt * ROWS + sub * RPW + slot / ZG;
+    const bool ok = row < n_rows;
+    const int t = ok ? udiv(row, p.div_g) : 0, h = hk * p.G + (ok ? row - t * p.G : 0);
+    const int64_t at = (int64_t)(sp.tok0 + t) * p.H + h;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    if (ok) {
       if constexpr (SOFTMAX) {
-        float m = -INFINITY, l = 0.f;
-        for (int z = 0; z < used; ++z) m = fmaxf(m, p.part_ml[2 * (z * th + at)]);
-        for (int z = 0; z < used; ++z) {
+#pragma unroll 4
+        for (int z = zi; z < used; z += ZG) m = fmaxf(m, p.part_ml[2 * (z * th + at)]);
+#pragma unroll 4
+        for (int z = zi; z < used; z += ZG) {
           const float mz = p.part_ml[2 * (z * th + at)];
           const float w = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - m);
           l = __builtin_fmaf(w, p.part_ml[2 * (z * th + at) + 1], l);
+          // a part that saw no key has zeros
           sum += w * *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
         }
-        f = l != 0.f ? 1.f / l : 0.f;
       } else {
-        for (int z = 0; z < used; ++z) sum += *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+#pragma unroll 4
+        for (int z = zi; z < used; z += ZG) sum += *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
       }
+    }
+    if constexpr (ZG > 1) {
+      sum_s[threadIdx.x] = sum;
+      if (d == 0) {
+        ml_s[slot][0] = m;
+        ml_s[slot][1] = l;
+      }
+      __syncthreads();
+      if (zi == 0) {
+        float all = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < ZG; ++g) all = fmaxf(all, ml_s[slot + g][0]);
+        sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        l = 0.f;
+#pragma unroll
+        for (int g = 0; g < ZG; ++g) {
+          const float mg = ml_s[slot + g][0];
+          const float w = !SOFTMAX ? 1.f : mg == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mg - all);
+          l = __builtin_fmaf(w, ml_s[slot + g][1], l);
+          sum += w * sum_s[threadIdx.x + g * LPR];
+        }
+      }
+      __syncthreads();
+    }
+    if (ok && zi == 0) {
+      const float f = !SOFTMAX ? p.post_scale : l != 0.f ? 1.f / l : 0.f;
       *(cu32x2_t*)(p.o + (int64_t)(sp.tok0 + t) * p.o_st + (int64_t)h * p.o_sh + d) =
           cu32x2_t{cpack(sum[0] * f, sum[1] * f), cpack(sum[2] * f, sum[3] * f)};
     }
   }
 }
-
 
 constexpr int64_t kMaxSeq = (int64_t)1 << 28;
 constexpr int kCUs = 256;  // MI355X compute units
@@ -130,16 +162,28 @@ CacheMask mask_of(const chia_attn_args* t) {
   return m;
 }
 
-template <int D, bool SOFTMAX>
-CacheAttnFn merge_of(int tile) {
-  return tile == CACHE_ROWS16 ? cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS16]>
-         : tile == CACHE_ROWS32 ? cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS32]>
-                                : cache_merge_kernel<D, SOFTMAX, kCacheRows[CACHE_ROWS128]>;
+struct Merge {
+  CacheAttnFn fn;
+  int subs;  // workgroups per row tile
+};
+
+template <int D, bool SOFTMAX, int ROWS>
+Merge merge_of(bool many) {
+  constexpr int slots = 1024 / D;
+  return many ? Merge{cache_merge_kernel<D, SOFTMAX, ROWS, 8>, ROWS * 8 / slots}
+              : Merge{cache_merge_kernel<D, SOFTMAX, ROWS, 1>, ROWS / slots};
 }
 
-CacheAttnFn merge_kernel(int head_dim, bool softmax, int tile) {
-  return head_dim == 64 ? (softmax ? merge_of<64, true>(tile) : merge_of<64, false>(tile))
-                        : (softmax ? merge_of<128, true>(tile) : merge_of<128, false>(tile));
+template <int D, bool SOFTMAX>
+Merge merge_of(int tile, bool many) {
+  return tile == CACHE_ROWS16 ? merge_of<D, SOFTMAX, kCacheRows[CACHE_ROWS16]>(many)
+         : tile == CACHE_ROWS32 ? merge_of<D, SOFTMAX, kCacheRows[CACHE_ROWS32]>(many)
+                                : merge_of<D, SOFTMAX, kCacheRows[CACHE_ROWS128]>(many);
+}
+
+Merge merge_kernel(int head_dim, bool softmax, int tile, bool many) {
+  return head_dim == 64 ? (softmax ? merge_of<64, true>(tile, many) : merge_of<64, false>(tile, many))
+                        : (softmax ? merge_of<128, true>(tile, many) : merge_of<128, false>(tile, many));
 }
 
 int64_t workspace_of(const chia_cache_attn_args* a, const Shape& s) {
@@ -222,7 +266,7 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
   p.part_o = (float*)a->workspace;
   p.part_ml = bytes > 0 ? p.part_o + s.parts * a->queries * t->heads * t->head_dim : nullptr;
   const int64_t units = t->batch * p.Hkv * s.tiles, wgs = units * s.parts;
-  if (wgs > INT32_MAX / 4) return CHIA_ATTN_ERR_SHAPE;
+  if (wgs > INT32_MAX / 4 || units > INT32_MAX / 64) return CHIA_ATTN_ERR_SHAPE;
 
   const int score = t->norm == CHIA_ATTN_NORM_SIGMOID ? CACHE_SIGMOID
                     : t->norm == CHIA_ATTN_NORM_RELU  ? CACHE_RELU
@@ -233,9 +277,11 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
   void* kargs[] = {&p};
   hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)wgs), dim3(256), kargs, 0,
                                    (hipStream_t)stream);
-  if (err == hipSuccess && s.parts > 1)
-    err = hipLaunchKernel(reinterpret_cast<const void*>(merge_kernel((int)t->head_dim, t->norm == CHIA_ATTN_NORM_SOFTMAX, s.tile)), dim3((unsigned)units), dim3(256), kargs, 0,
+  if (err == hipSuccess && s.parts > 1) {
+    const Merge m = merge_kernel((int)t->head_dim, t->norm == CHIA_ATTN_NORM_SOFTMAX, s.tile, s.parts >= 8);
+    err = hipLaunchKernel(reinterpret_cast<const void*>(m.fn), dim3((unsigned)(units * m.subs)), dim3(256), kargs, 0,
                           (hipStream_t)stream);
+  }
   if (err != hipSuccess) return (int)err;
   err = hipGetLastError();
   return err == hipSuccess ? CHIA_ATTN_OK : (int)err;

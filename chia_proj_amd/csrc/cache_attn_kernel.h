@@ -123,15 +123,14 @@ __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0
 template <int D>
 struct CacheKeys {
   cu32x4_t w[2][D / 64];
-  int32_t key;  // first key
-  float scale[2];
-  bool ok[2];   // the page is inside the cache
+  int32_t key;     // first key
+  int32_t at[2];   // lane that holds the half's page
+  bool ok[2];      // the page is inside the cache
 };
 
 template <int D>
 struct CacheValues {
   uint32_t w[8][D / 64];
-  float scale[2];
 };
 
 template <int D, int FMT, int SCORE, int NT, bool SPLIT>
@@ -150,10 +149,25 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
   const int z = (int)blockIdx.x - u * p.parts;
   const int rh = udiv(u, p.div_tiles), rt0 = u - rh * p.tiles;
   const int r = udiv(rh, p.div_hkv), hk = rh - r * p.Hkv;
-  const CacheSpan sp = cache_span(p, r);
-  const int n_rows = sp.n * p.G;
   const int bs_mask = (1 << p.bshift) - 1;
   const int32_t* table = p.table + (int64_t)r * p.table_stride;
+  // The chain lengths -> table -> scales, keys is what a short request waits for.
+  // Without a window the first pages follow from the launch alone, so they are
+  // asked for before the length is there (a wrong guess is only asked again).
+  int32_t pg0 = 1 << 30, pg_id = -1;
+  float pg_ks = 0.f, pg_vs = 0.f;
+  if (p.mask.window == 0 && p.mask.blk == 0) {
+    int first = z * p.chunk;
+    if (SPLIT && ((p.chunk * kStepKeys) >> p.bshift) > 63) first += wave * ((p.chunk + 3) >> 2);
+    pg0 = (first * kStepKeys) >> p.bshift;
+    const int at = pg0 + lane;
+    pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
+    const int64_t id = imax32(pg_id, 0);
+    pg_ks = p.ks[id * p.ks_sb + hk * p.ks_sh];
+    pg_vs = p.vs[id * p.vs_sb + hk * p.vs_sh];
+  }
+  const CacheSpan sp = cache_span(p, r);
+  const int n_rows = sp.n * p.G;
 
   for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
     const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
@@ -205,9 +219,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       for (int c = 0; c < DC; ++c) acc[b][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // page numbers and scales of 64 pages in a row, one per lane
-    int32_t pg0 = -(1 << 30), pg_id = 0;
-    float pg_ks = 0.f, pg_vs = 0.f;
+    // Page numbers and scales of 64 pages from pg0 on, one per lane; a step's two
+    // halves are always among them.
     auto pages_from = [&](int pg) {
       pg0 = pg;
       const int at = pg + lane;
@@ -218,35 +231,32 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     };
     const uint32_t k_off = (uint32_t)(n16 * (int32_t)p.k_st + 16 * g);
     const uint32_t v_off = (uint32_t)(4 * g * (int32_t)p.v_st + n16 * DC);
-
-    // page (uniform; -1 outside the cache) of key j
-    auto lane_of = [&](int j) {
-      const int pg = j >> p.bshift;
-      if ((uint32_t)(pg - pg0) >= 64u) pages_from(pg);
-      return pg - pg0;
+    auto pages_of = [&](int key) {
+      const int pg = key >> p.bshift, last = (key + 16) >> p.bshift;
+      if (pg < pg0 || last - pg0 > 63) pages_from(pg);
     };
     CacheKeys<D> kk;
     CacheValues<D> vv;
     auto issue_k = [&](int s) {
       kk.key = walk_key(tw, s);
+      pages_of(kk.key);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int j = kk.key + 16 * t, at = lane_of(j);
+        const int j = kk.key + 16 * t, at = (j >> p.bshift) - pg0;
         const int id = __builtin_amdgcn_readlane(pg_id, at);
-        kk.scale[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_ks), at));
+        kk.at[t] = at;
         kk.ok[t] = id >= 0;
         const uint8_t* kp = p.k + (int64_t)imax32(id, 0) * p.k_sb + hk * p.k_sh + (int64_t)(j & bs_mask) * p.k_st;
 #pragma unroll
         for (int c = 0; c < W64; ++c) kk.w[t][c] = *(const cu32x4_t*)(kp + k_off + 64 * c);
       }
     };
-    auto issue_v = [&](int s) {
+    auto issue_v = [&](int s) {  // after issue_k of the same step
       const int key = walk_key(tw, s);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int j = key + 16 * t, at = lane_of(j);
+        const int j = key + 16 * t, at = (j >> p.bshift) - pg0;
         const int id = __builtin_amdgcn_readlane(pg_id, at);
-        vv.scale[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_vs), at));
         const uint8_t* vp = p.v + (int64_t)imax32(id, 0) * p.v_sb + hk * p.v_sh + (int64_t)(j & bs_mask) * p.v_st;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -267,13 +277,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     // rows that see them is added first: NaN where a row sees a NaN (a product of
     // 1 at those codes with 1 at the keys that it sees), and an infinity of e5m2,
     // as 2^120, by the row's weights, grown until it is one.
-    auto clean = [&](const uint32_t (&vis)[NT], const uint32_t (&pw)[NT][4], float (&v2)[2]) {
+    auto clean = [&](const uint32_t (&vis)[NT], const uint32_t (&pw)[NT][4], const float (&vs)[2], float (&v2)[2]) {
       uint32_t bad = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
 #pragma unroll
         for (int w = 0; w < W64; ++w) bad |= nonfinite<FMT>(vv.w[e][w]);
-      const bool bs2[2] = {!(fabsf(vv.scale[0]) < INFINITY), !(fabsf(vv.scale[1]) < INFINITY)};
+      const bool bs2[2] = {!(fabsf(vs[0]) < INFINITY), !(fabsf(vs[1]) < INFINITY)};
       if (!__any(bad != 0) && !bs2[0] && !bs2[1]) return;
       cbf16x8_t sees[NT];
 #pragma unroll
@@ -333,7 +343,12 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     auto compute = [&](int s) {
       f32x4_t sc[NT][2];  // lane: row n16 of each block, keys key + 16 t + 4 g + e
       const int key = kk.key;
-      const float ks[2] = {kk.scale[0], kk.scale[1]};
+      float ks[2], vs[2];  // before the next step's pages take their place
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_ks), kk.at[t]));
+        vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_vs), kk.at[t]));
+      }
       const bool pok[2] = {kk.ok[0], kk.ok[1]};
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -355,7 +370,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       float v2[2], mant[2], inv[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const uint32_t bits = __float_as_uint(vv.scale[t]);
+        const uint32_t bits = __float_as_uint(vs[t]);
         v2[t] = __uint_as_float(bits & 0x7f800000u);
         mant[t] = __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
       }
@@ -457,7 +472,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
             l_run[b] = __builtin_fmaf(add, inv[t], l_run[b]);
           }
       }
-      if (!full) clean(vis, pw, v2);
+      if (!full) clean(vis, pw, vs, v2);
 #pragma unroll
       for (int w = 0; w < W64; ++w) {
         cu32x4_t va[4];
