@@ -140,11 +140,30 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   const TileWalk w = cache_tile_walk(m, i0 < 0 ? 0 : i0, (int32_t)S - 1, (int32_t)S);
   const int64_t steps = w.n > 0 ? w.n : 1;
   const int64_t groups = t->batch * hkv * s.tiles;
-  // Enough workgroups for two rounds of three per CU, each with two steps or more per wavefront.
-  const int64_t want = (6 * kCUs + groups - 1) / groups;
-  const int64_t least = s.tile == CACHE_ROWS128 ? 16 : 8;
-  s.chunk = (steps + want - 1) / want;
-  if (s.chunk < least) s.chunk = least;
+  // How many parts.  A part costs a workgroup's start and end (lengths, table, first
+  // keys; merge) whatever it holds, the second kernel 3 to 5 us, and too few parts
+  // leave CUs idle or waiting for the longest request.  With `room` the workgroups
+  // that the chip holds at once:
+  //   * 16-row tiles, up to 128 (request, head) pairs: 3/4 of room, since their parts
+  //     are nearly equal (2 requests of 131072 tokens, H32/8 D128, us by workgroups asked for:
+  //     100 (512), 103 (768), 109 (1024); 11 of up to 32318, H16/8 D64: 90, 68, 70); beyond,
+  //     3/2 of it, since many of their parts do not exist (16 of 33 .. 4096, 16 heads, D64: 38 (512), 33 (1024),
+  //     28 (1536), 33 (2048));
+  //   * two workgroups per CU: room (16 requests verifying 5 tokens over 4096, H32/8 D128: 35 (512), 42, 47);
+  //   * parts of 16 steps (512 keys) or more, of 8 where that is a handful of workgroups
+  //     (2 of 2994, 2 heads: 13.1 -> 11.6);
+  //   * but, for balance, no parts much beyond 48 steps (64 of 97 .. 8192, H32/8 D128: 125 (1 part),
+  //     113 (4), 106 (5), 108 (6)).
+  const bool small = s.tile == CACHE_ROWS16;
+  const int64_t room = kCUs * (small ? (t->head_dim == 64 ? 4 : 3) : 2);
+  const int64_t least = groups * steps <= 2048 && steps > 32 && small ? 8 : 16;
+  int64_t parts = (!small ? room : groups <= 128 ? room * 3 / 4 : room * 3 / 2) / groups;
+  if (parts > steps / least) parts = steps / least;
+  int64_t balance = steps / 48;
+  if (balance > 6 * room / groups) balance = 6 * room / groups;
+  if (parts < balance && groups > 128) parts = balance;
+  if (parts < 1) parts = 1;
+  s.chunk = (steps + parts - 1) / parts;
   s.parts = (steps + s.chunk - 1) / s.chunk;
   return s;
 }
@@ -255,7 +274,6 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
   p.tiles = (int32_t)s.tiles;
   p.parts = (int32_t)s.parts;
   p.chunk = (int32_t)s.chunk;
-  p.div_parts = make_udiv(p.parts);
   p.div_tiles = make_udiv(p.tiles);
   p.div_hkv = make_udiv(p.Hkv);
   p.div_g = make_udiv(p.G);
@@ -267,6 +285,8 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
   p.part_ml = bytes > 0 ? p.part_o + s.parts * a->queries * t->heads * t->head_dim : nullptr;
   const int64_t units = t->batch * p.Hkv * s.tiles, wgs = units * s.parts;
   if (wgs > INT32_MAX / 4 || units > INT32_MAX / 64) return CHIA_ATTN_ERR_SHAPE;
+  p.units = (int32_t)units;
+  p.div_units = make_udiv(p.units);
 
   const int score = t->norm == CHIA_ATTN_NORM_SIGMOID ? CACHE_SIGMOID
                     : t->norm == CHIA_ATTN_NORM_RELU  ? CACHE_RELU

@@ -57,7 +57,8 @@ struct CacheAttnParams {
   CacheMask mask;
   int32_t R, H, Hkv, G, T, width, num_blocks, bshift;
   int32_t tiles, parts, chunk;  // row tiles and key parts per (request, K/V head); steps per part
-  UDiv div_parts, div_tiles, div_hkv, div_g;
+  int32_t units;                 // R Hkv tiles
+  UDiv div_units, div_tiles, div_hkv, div_g;
   float scale, softcap, bias, post_scale;
   float* part_o;   // [parts, T H, D]
   float* part_ml;  // [parts, T H, 2]: running max (log2), row sum
@@ -145,8 +146,12 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
 
   const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int u = udiv((int)blockIdx.x, p.div_parts);
-  const int z = (int)blockIdx.x - u * p.parts;
+  // Parts in the slowest place: workgroups next to each other, which go to the XCDs
+  // in turn, then are of different requests and heads.  (With parts next to each
+  // other and 4 or 8 of them, some XCDs got only first parts and some only last
+  // ones, which short requests do not have: 64 requests of 97 .. 8192 tokens in 4
+  // parts, H32/8 D128, 137 us.)
+  const int z = udiv((int)blockIdx.x, p.div_units), u = (int)blockIdx.x - z * p.units;
   const int rh = udiv(u, p.div_tiles), rt0 = u - rh * p.tiles;
   const int r = udiv(rh, p.div_hkv), hk = rh - r * p.Hkv;
   const int bs_mask = (1 << p.bshift) - 1;
