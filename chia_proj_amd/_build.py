@@ -23,8 +23,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 BUILD_DIR = REPO_DIR / "_build"
 
 SOURCES = ["attn_fwd_d64.hip", "attn_fwd_d128.hip", "attn_fwd_q1_d64.hip", "attn_fwd_q1_d128.hip", "attn_bwd_d64.hip", "attn_bwd_d128.hip", "attn_fp8.hip", "attn_api.hip",
-           "cache_attn_d64.hip", "cache_attn_d128.hip", "cache_attn.hip", "cache_write.hip", "cache_tables.hip"]
-HEADERS = ["attn_fwd_kernel.h", "attn_fwd_q1_kernel.h", "lds_layout.h", "mask.h", "cache_geom.h", "cache_attn_kernel.h"]
+           "cache_attn_d64.hip", "cache_attn_d128.hip", "cache_prompt.hip", "cache_attn.hip", "cache_write.hip", "cache_tables.hip"]
+HEADERS = ["attn_fwd_kernel.h", "attn_fwd_q1_kernel.h", "lds_layout.h", "mask.h", "cache_geom.h", "cache_attn_kernel.h", "cache_prompt_kernel.h"]
 
 ARCH = "gfx950"
 HIPCC_FLAGS = [

@@ -137,7 +137,7 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   const int64_t S = t->seqlen < (a->width * a->block_size) ? t->seqlen : a->width * a->block_size;
   const int64_t span = (R + G - 1) / G;
   const int32_t i0 = (int32_t)(S - (span < most ? span : most));
-  const TileWalk w = cache_tile_walk(m, i0 < 0 ? 0 : i0, (int32_t)S - 1, (int32_t)S);
+  const TileWalk w = cache_tile_walk(m, i0 < 0 ? 0 : i0, (int32_t)S - 1, (int32_t)S, kCacheStep[s.tile]);
   const int64_t steps = w.n > 0 ? w.n : 1;
   const int64_t groups = t->batch * hkv * s.tiles;
   // How many parts.  A part costs a workgroup's start and end (lengths, table, first
@@ -161,7 +161,7 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   if (parts > steps / least) parts = steps / least;
   int64_t balance = steps / 48;
   if (balance > 6 * room / groups) balance = 6 * room / groups;
-  if (parts < balance && groups > 128) parts = balance;
+  if (s.tile != CACHE_ROWS128 && parts < balance && groups > 128) parts = balance;
   if (parts < 1) parts = 1;
   s.chunk = (steps + parts - 1) / parts;
   s.parts = (steps + s.chunk - 1) / s.chunk;
@@ -291,8 +291,9 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
   const int score = t->norm == CHIA_ATTN_NORM_SIGMOID ? CACHE_SIGMOID
                     : t->norm == CHIA_ATTN_NORM_RELU  ? CACHE_RELU
                     : t->alibi_slopes || t->softcap > 0.f ? CACHE_SOFTMAX_MOD : CACHE_SOFTMAX;
-  const CacheAttnFn fn = t->head_dim == 64 ? select_cache_kernel_d64((int)a->format, score, s.tile)
-                                           : select_cache_kernel_d128((int)a->format, score, s.tile);
+  const CacheAttnFn fn = s.tile == CACHE_ROWS128 ? select_cache_prompt_kernel((int)t->head_dim, (int)a->format, score)
+                         : t->head_dim == 64     ? select_cache_kernel_d64((int)a->format, score, s.tile)
+                                                 : select_cache_kernel_d128((int)a->format, score, s.tile);
   if (!fn) return CHIA_ATTN_ERR_NORM;
   void* kargs[] = {&p};
   hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)wgs), dim3(256), kargs, 0,

@@ -22,11 +22,10 @@
 // sum adds the rounded weights.  The softmax maximum moves only when a score
 // exceeds it by more than 8 (log2), which one vote per step finds out.
 //
-// Rows come in tiles of 16 NT per wavefront.  SPLIT: the four wavefronts of a
-// workgroup split the keys of one tile and merge through LDS.  Otherwise
-// (prompts) each has rows of its own and the shared K / V pieces come from the
-// cache hierarchy.  Keys of a tile are further split over workgroups
-// (cache_geom.h); their partial rows are merged by a second kernel.
+// Rows come in tiles of 16 NT; the four wavefronts of a workgroup split a tile's
+// keys and merge through LDS.  The keys are further split over workgroups
+// (cache_geom.h), whose partial rows a second kernel joins.  Prompts, with many
+// rows to a K/V head, have a kernel of their own (cache_prompt_kernel.h).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -91,7 +90,7 @@ template <int ROWS>
 __device__ __forceinline__ TileWalk cache_walk_of(const CacheAttnParams& p, const CacheSpan& s, int rt) {
   const int t0 = udiv(rt * ROWS, p.div_g), t1 = imin32(udiv(rt * ROWS + ROWS - 1, p.div_g), s.n - 1);
   const int32_t at = s.S - s.n;
-  return cache_tile_walk(p.mask, at + t0, at + t1, s.S);
+  return cache_tile_walk(p.mask, at + t0, at + t1, s.S, ROWS == 128 ? 64 : 32);
 }
 
 template <int FMT, bool HI>
@@ -134,15 +133,15 @@ struct CacheValues {
   uint32_t w[8][D / 64];
 };
 
-template <int D, int FMT, int SCORE, int NT, bool SPLIT>
+template <int D, int FMT, int SCORE, int NT>
 __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const CacheAttnParams p) {
   constexpr int KS = D / 32;            // k-steps of the first product
   constexpr int DC = D / 16;            // 16-row blocks of O^T; columns per lane of V
   constexpr int W64 = D / 64;
-  constexpr int ROWS_W = 16 * NT, ROWS = SPLIT ? ROWS_W : 4 * ROWS_W;
+  constexpr int ROWS = 16 * NT;
   constexpr bool SOFTMAX = SCORE == CACHE_SOFTMAX || SCORE == CACHE_SOFTMAX_MOD;
   constexpr int LP = D + 4;             // LDS row pitch: rows start in other banks
-  __shared__ __attribute__((aligned(16))) float lds[SPLIT ? 4 * ROWS_W * LP + 4 * ROWS_W * 2 : 1];
+  __shared__ __attribute__((aligned(16))) float lds[4 * ROWS * LP + 4 * ROWS * 2];
 
   const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -163,8 +162,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
   float pg_ks = 0.f, pg_vs = 0.f;
   if (p.mask.window == 0 && p.mask.blk == 0) {
     int first = z * p.chunk;
-    if (SPLIT && ((p.chunk * kStepKeys) >> p.bshift) > 63) first += wave * ((p.chunk + 3) >> 2);
-    pg0 = (first * kStepKeys) >> p.bshift;
+    if (((p.chunk * 32) >> p.bshift) > 63) first += wave * ((p.chunk + 3) >> 2);
+    pg0 = (first * 32) >> p.bshift;
     const int at = pg0 + lane;
     pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
     const int64_t id = imax32(pg_id, 0);
@@ -180,12 +179,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     const int used = (tw.n + chunk - 1) / chunk;  // parts that have steps
     if (z > 0 && z >= used) continue;             // part 0 writes the rows that see nothing
     int s0 = z * chunk, s1 = imin32(s0 + chunk, tw.n);
-    const int row0 = rt * ROWS + (SPLIT ? 0 : wave * ROWS_W);
-    if constexpr (SPLIT) {
-      const int per = (s1 - s0 + 3) >> 2;
-      s0 = imin32(s0 + wave * per, s1);
-      s1 = imin32(s0 + per, s1);
-    }
+    const int row0 = rt * ROWS, per = (s1 - s0 + 3) >> 2;
+    s0 = imin32(s0 + wave * per, s1);
+    s1 = imin32(s0 + per, s1);
 
     // this lane's rows (one per 16-row block): keys, score constants, Q
     RowKeys rk[NT];
@@ -517,139 +513,101 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       }
 
     const bool whole = used <= 1;  // this workgroup has all the keys of its rows
-    // One lane's outputs of block b: d = DC (4 g + e) + c.
-    auto store = [&](int b, float factor, float m, float l) {
-      if (!rok[b]) return;
-      if (whole) {
-        uint16_t* op = p.o + (int64_t)otok[b] * p.o_st + (int64_t)ohead[b] * p.o_sh;
+    // merge the four wavefronts' keys
+    float* ml = lds + 4 * ROWS * LP;  // [4][ROWS][2]
+    if constexpr (SOFTMAX) {
+      if (g == 0)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w[DC / 2];
-#pragma unroll
-          for (int c = 0; c < DC / 2; ++c) w[c] = cpack(acc[b][2 * c][e] * factor, acc[b][2 * c + 1][e] * factor);
-          uint16_t* at = op + DC * (4 * g + e);
-          if constexpr (DC == 8) *(cu32x4_t*)at = cu32x4_t{w[0], w[1], w[2], w[3]};
-          else *(cu32x2_t*)at = cu32x2_t{w[0], w[1]};
+        for (int b = 0; b < NT; ++b) {
+          ml[(wave * ROWS + 16 * b + n16) * 2] = m_run[b];
+          ml[(wave * ROWS + 16 * b + n16) * 2 + 1] = l_run[b];
         }
+    }
+    __syncthreads();
+    float m_all[NT], l_all[NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+      m_all[b] = -INFINITY;
+      l_all[b] = 0.f;
+      if constexpr (SOFTMAX) {
+        float mw[4], lw[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          mw[w] = ml[(w * ROWS + 16 * b + n16) * 2];
+          lw[w] = ml[(w * ROWS + 16 * b + n16) * 2 + 1];
+          m_all[b] = fmaxf(m_all[b], mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          l_all[b] += mw[w] == -INFINITY ? 0.f : lw[w] * __builtin_amdgcn_exp2f(mw[w] - m_all[b]);
+        const float f = m_run[b] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[b] - m_all[b]);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) acc[b][c] *= f;
+      }
+      // [wave][row][d], the pieces of a lane 16 bytes each
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < DC; c += 4)
+          *(f32x4_t*)(lds + (wave * ROWS + 16 * b + n16) * LP + DC * (4 * g + e) + c) =
+              f32x4_t{acc[b][c][e], acc[b][c + 1][e], acc[b][c + 2][e], acc[b][c + 3][e]};
+    }
+    __syncthreads();
+    // wavefront w stores the pieces e = w of every lane's rows
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+      f32x4_t sum[DC / 4];
+#pragma unroll
+      for (int c = 0; c < DC / 4; ++c) {
+        sum[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          sum[c] += *(const f32x4_t*)(lds + (w * ROWS + 16 * b + n16) * LP + DC * (4 * g + wave) + 4 * c);
+      }
+      if (!rok[b]) continue;
+      const int at = DC * (4 * g + wave);
+      if (whole) {
+        const float f = SOFTMAX ? (l_all[b] != 0.f ? 1.f / l_all[b] : 0.f) : p.post_scale;
+        uint16_t* op = p.o + (int64_t)otok[b] * p.o_st + (int64_t)ohead[b] * p.o_sh + at;
+        if constexpr (DC == 8)
+          *(cu32x4_t*)op = cu32x4_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f),
+                                    cpack(sum[1][0] * f, sum[1][1] * f), cpack(sum[1][2] * f, sum[1][3] * f)};
+        else
+          *(cu32x2_t*)op = cu32x2_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f)};
       } else {
         const int64_t row = ((int64_t)z * p.T + otok[b]) * p.H + ohead[b];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int c = 0; c < DC; c += 4)
-            *(f32x4_t*)(p.part_o + row * D + DC * (4 * g + e) + c) =
-                f32x4_t{acc[b][c][e], acc[b][c + 1][e], acc[b][c + 2][e], acc[b][c + 3][e]};
-        if (SOFTMAX && g == 0) {
-          p.part_ml[2 * row] = m;
-          p.part_ml[2 * row + 1] = l;
+        for (int c = 0; c < DC / 4; ++c) *(f32x4_t*)(p.part_o + row * D + at + 4 * c) = sum[c];
+        if (SOFTMAX && g == 0 && wave == 0) {
+          p.part_ml[2 * row] = m_all[b];
+          p.part_ml[2 * row + 1] = l_all[b];
         }
       }
-    };
-
-    if constexpr (!SPLIT) {
-#pragma unroll
-      for (int b = 0; b < NT; ++b)
-        store(b, SOFTMAX ? (l_run[b] != 0.f ? 1.f / l_run[b] : 0.f) : p.post_scale, m_run[b], l_run[b]);
-    } else {
-      // merge the four wavefronts' keys
-      float* ml = lds + 4 * ROWS_W * LP;  // [4][ROWS_W][2]
-      if constexpr (SOFTMAX) {
-        __syncthreads();  // the tile before has been read
-        if (g == 0)
-#pragma unroll
-          for (int b = 0; b < NT; ++b) {
-            ml[(wave * ROWS_W + 16 * b + n16) * 2] = m_run[b];
-            ml[(wave * ROWS_W + 16 * b + n16) * 2 + 1] = l_run[b];
-          }
-      }
-      __syncthreads();
-      float m_all[NT], l_all[NT];
-#pragma unroll
-      for (int b = 0; b < NT; ++b) {
-        m_all[b] = -INFINITY;
-        l_all[b] = 0.f;
-        if constexpr (SOFTMAX) {
-          float mw[4], lw[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            mw[w] = ml[(w * ROWS_W + 16 * b + n16) * 2];
-            lw[w] = ml[(w * ROWS_W + 16 * b + n16) * 2 + 1];
-            m_all[b] = fmaxf(m_all[b], mw[w]);
-          }
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            l_all[b] += mw[w] == -INFINITY ? 0.f : lw[w] * __builtin_amdgcn_exp2f(mw[w] - m_all[b]);
-          const float f = m_run[b] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[b] - m_all[b]);
-#pragma unroll
-          for (int c = 0; c < DC; ++c) acc[b][c] *= f;
-        }
-        // [wave][row][d], the pieces of a lane 16 bytes each
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int c = 0; c < DC; c += 4)
-            *(f32x4_t*)(lds + (wave * ROWS_W + 16 * b + n16) * LP + DC * (4 * g + e) + c) =
-                f32x4_t{acc[b][c][e], acc[b][c + 1][e], acc[b][c + 2][e], acc[b][c + 3][e]};
-      }
-      __syncthreads();
-      // wavefront w stores the pieces e = w of every lane's rows
-#pragma unroll
-      for (int b = 0; b < NT; ++b) {
-        f32x4_t sum[DC / 4];
-#pragma unroll
-        for (int c = 0; c < DC / 4; ++c) {
-          sum[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            sum[c] += *(const f32x4_t*)(lds + (w * ROWS_W + 16 * b + n16) * LP + DC * (4 * g + wave) + 4 * c);
-        }
-        if (!rok[b]) continue;
-        const int at = DC * (4 * g + wave);
-        if (whole) {
-          const float f = SOFTMAX ? (l_all[b] != 0.f ? 1.f / l_all[b] : 0.f) : p.post_scale;
-          uint16_t* op = p.o + (int64_t)otok[b] * p.o_st + (int64_t)ohead[b] * p.o_sh + at;
-          if constexpr (DC == 8)
-            *(cu32x4_t*)op = cu32x4_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f),
-                                      cpack(sum[1][0] * f, sum[1][1] * f), cpack(sum[1][2] * f, sum[1][3] * f)};
-          else
-            *(cu32x2_t*)op = cu32x2_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f)};
-        } else {
-          const int64_t row = ((int64_t)z * p.T + otok[b]) * p.H + ohead[b];
-#pragma unroll
-          for (int c = 0; c < DC / 4; ++c) *(f32x4_t*)(p.part_o + row * D + at + 4 * c) = sum[c];
-          if (SOFTMAX && g == 0 && wave == 0) {
-            p.part_ml[2 * row] = m_all[b];
-            p.part_ml[2 * row + 1] = l_all[b];
-          }
-        }
-      }
-      __syncthreads();  // the next tile writes the same LDS
     }
+    __syncthreads();  // the next tile writes the same LDS
   }
 }
 
 using CacheAttnFn = void (*)(CacheAttnParams);
 
-// The three row tiles: 16 or 32 rows whose keys the wavefronts split, or 32 rows a wavefront.
+// The row tiles: 16 or 32 rows whose keys the wavefronts split (this file), 128 rows (cache_prompt_kernel.h).
 enum CacheTile : int { CACHE_ROWS16 = 0, CACHE_ROWS32 = 1, CACHE_ROWS128 = 2 };
-constexpr int kCacheRows[3] = {16, 32, 128};
+constexpr int kCacheRows[3] = {16, 32, 128}, kCacheStep[3] = {32, 32, 64};
 
 CacheAttnFn select_cache_kernel_d64(int format, int score, int tile);
 CacheAttnFn select_cache_kernel_d128(int format, int score, int tile);
+CacheAttnFn select_cache_prompt_kernel(int head_dim, int format, int score);
 
 template <int D>
 CacheAttnFn pick_cache_kernel(int format, int score, int tile) {
-#define CHIA_CACHE(F, S, T, N, P) \
-  if (format == F && score == S && tile == T) return cache_attn_kernel<D, F, S, N, P>;
-#define CHIA_CACHE_TILES(F, S) \
-  CHIA_CACHE(F, S, CACHE_ROWS16, 1, true) CHIA_CACHE(F, S, CACHE_ROWS32, 2, true) CHIA_CACHE(F, S, CACHE_ROWS128, 2, false)
-#define CHIA_CACHE_FMT(F)                                                              \
-  CHIA_CACHE_TILES(F, CACHE_SOFTMAX) CHIA_CACHE_TILES(F, CACHE_SOFTMAX_MOD)            \
-  CHIA_CACHE_TILES(F, CACHE_SIGMOID) CHIA_CACHE_TILES(F, CACHE_RELU)
+#define CHIA_CACHE(F, S)                                                                          \
+  if (format == F && score == S)                                                                  \
+    return tile == CACHE_ROWS16 ? cache_attn_kernel<D, F, S, 1> : cache_attn_kernel<D, F, S, 2>;
+#define CHIA_CACHE_FMT(F) \
+  CHIA_CACHE(F, CACHE_SOFTMAX) CHIA_CACHE(F, CACHE_SOFTMAX_MOD) CHIA_CACHE(F, CACHE_SIGMOID) CHIA_CACHE(F, CACHE_RELU)
   CHIA_CACHE_FMT(0)
   CHIA_CACHE_FMT(1)
 #undef CHIA_CACHE_FMT
-#undef CHIA_CACHE_TILES
 #undef CHIA_CACHE
   return nullptr;
 }

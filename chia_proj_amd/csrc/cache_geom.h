@@ -5,8 +5,8 @@
 // For one query at position i of a request with S tokens the mask of mask.h is
 //   visible(j) = j < S and (j < pre  or  (lo <= j < hi and (i - j) % dil == 0)).
 // A row tile holds queries at positions i0 .. i1 (times the query heads of one
-// K/V head).  Its keys are walked in steps of 32: the prefix's steps, then those
-// of the band that lie behind them.  The steps are split evenly enough: `parts`
+// K/V head).  Its keys are walked in steps of 32 or 64: the prefix's steps, then
+// those of the band that lie behind them.  The steps are split evenly enough: `parts`
 // workgroups take `chunk` steps each, chunk being the launch's, or more where a
 // request is longer than the launch was told.
 #pragma once
@@ -14,7 +14,6 @@
 
 namespace chia {
 
-constexpr int kStepKeys = 32;
 
 // A table's page number, or -1 for one outside the cache: such a page is not read.
 CHIA_HD int32_t cache_page(int32_t id, int32_t num_blocks) { return (uint32_t)id < (uint32_t)num_blocks ? id : -1; }
@@ -47,20 +46,22 @@ CHIA_HD RowKeys cache_row_keys(const CacheMask& m, int32_t i, int32_t S) {
   return {lo, hi, imin32(m.prefix, S)};
 }
 
-// The walk of a row tile: step s covers keys key_of(s) .. + 31.
+// The walk of a row tile: step s covers the `step` keys from walk_key(s) on.
 struct TileWalk {
+  int32_t step;
   int32_t n_pre, first, n;          // prefix steps, first band step, steps in all
   int32_t full_lo, full_hi, full_pre;  // every row sees [full_lo, full_hi) and [0, full_pre) (dilation 1)
 };
 
-CHIA_HD TileWalk cache_tile_walk(const CacheMask& m, int32_t i0, int32_t i1, int32_t S) {
+CHIA_HD TileWalk cache_tile_walk(const CacheMask& m, int32_t i0, int32_t i1, int32_t S, int32_t step) {
   // lo and hi never fall with the position: the first row reaches lowest, the last highest.
   const RowKeys a = cache_row_keys(m, imax32(i0, 0), S), b = cache_row_keys(m, i1, S);
   TileWalk w;
+  w.step = step;  // a power of two known to the compiler where this is called
   const int32_t pre = b.pre;
-  w.n_pre = (pre + kStepKeys - 1) / kStepKeys;
-  w.first = imax32(w.n_pre, a.lo / kStepKeys);
-  w.n = w.n_pre + imax32(0, (b.hi + kStepKeys - 1) / kStepKeys - w.first);
+  w.n_pre = (pre + step - 1) / step;
+  w.first = imax32(w.n_pre, a.lo / step);
+  w.n = w.n_pre + imax32(0, (b.hi + step - 1) / step - w.first);
   if (i1 < 0) w.n_pre = w.n = 0;
   w.full_lo = b.lo;
   w.full_hi = i0 < 0 || m.dil > 1 ? 0 : a.hi;
@@ -69,7 +70,7 @@ CHIA_HD TileWalk cache_tile_walk(const CacheMask& m, int32_t i0, int32_t i1, int
 }
 
 CHIA_HD int32_t walk_key(const TileWalk& w, int32_t s) {
-  return kStepKeys * (s < w.n_pre ? s : w.first + (s - w.n_pre));
+  return w.step * (s < w.n_pre ? s : w.first + (s - w.n_pre));
 }
 
 // Whether every row of the tile sees all of keys c .. c + n - 1.

@@ -1,0 +1,442 @@
+// cache_prompt_kernel.h -- attention of many queries over the paged 8-bit cache (gfx950).
+//
+// The function of cache_attn_kernel.h for prompts and chunks of them: with a
+// hundred rows and more to a K/V head the matrix products bind, not the codes'
+// bytes, so a workgroup converts each 64-key tile of K and V to bf16 once, in
+// LDS, for its 128 rows.
+//   S^T[key, row] = K Q^T, O^T[d, row] += V^T P^T on v_mfma_f32_32x32x16_bf16 with
+//   the operand layouts and LDS swizzle of the one-block forward core
+//   (attn_fwd_q1_kernel.h): a lane has one row and 16 keys of a 32-key block.
+// A thread loads 16 codes of one key per 256 chunks of the tile, one tile ahead of
+// the one computed, and stores them as 32 bytes of bf16 behind the current tile's
+// work (two LDS stages, one barrier per tile).  The power of two of a key's scale
+// is applied by the conversion; the fraction of a scale that is no power of two,
+// which a branch finds out, multiplies the scores (K) or the weights (V).
+#pragma once
+#include "attn_fwd_kernel.h"
+#include "cache_attn_kernel.h"
+
+namespace chia {
+
+template <int FMT>
+__device__ __forceinline__ cu32x4_t cvt8(uint32_t lo, uint32_t hi, float scale) {
+  return cu32x4_t{cvt2<FMT, false>(lo, scale), cvt2<FMT, true>(lo, scale), cvt2<FMT, false>(hi, scale), cvt2<FMT, true>(hi, scale)};
+}
+
+__device__ __forceinline__ float pow2_of(float s) { return __uint_as_float(__float_as_uint(s) & 0x7f800000u); }
+__device__ __forceinline__ float fraction_of(float s) { return __uint_as_float((__float_as_uint(s) & 0x807fffffu) | 0x3f800000u); }
+
+// One of two values (by value: chosen by reference they would have to lie in memory).
+template <class T>
+__device__ __forceinline__ T sel(int second, T a, T b) {
+  return second ? b : a;
+}
+
+// x, hidden from the compiler: addresses made from it stay where they are used
+// rather than in registers through the walk.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <int D, int FMT, int SCORE>
+__global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnParams p) {
+  constexpr int BN = 64, ROWS = 128;
+  constexpr int DK = D / 16, DB = D / 32;
+  constexpr int RP = 2 * D;                      // LDS row pitch (bytes)
+  constexpr int K_BYTES = BN * RP, STAGE = 2 * K_BYTES;
+  constexpr int CH = D / 16;                     // 16-code chunks per key
+  constexpr int NL = BN * CH / 256;              // chunks per thread (of K, and of V)
+  constexpr bool SOFTMAX = SCORE == CACHE_SOFTMAX || SCORE == CACHE_SOFTMAX_MOD;
+  typedef short i16x8_t __attribute__((ext_vector_type(8)));
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ int poison_s;                       // some tile's V had codes that are no numbers
+
+  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // parts in the slowest place, row tiles in the fastest (cache_attn_kernel.h says why; with each
+  // K/V head's tiles on one XCD, whose L2 would hold its keys, a chunk of two prompts took 871 us, not 654)
+  const int L = (int)blockIdx.x;
+  const int z = udiv(L, p.div_units), u = L - z * p.units;
+  const int rh = udiv(u, p.div_tiles), rt0 = u - rh * p.tiles;
+  const int r = udiv(rh, p.div_hkv), hk = rh - r * p.Hkv;
+  const CacheSpan sp = cache_span(p, r);
+  const int n_rows = sp.n * p.G;
+  const int bs_mask = (1 << p.bshift) - 1;
+  const int32_t* table = p.table + (int64_t)r * p.table_stride;
+  const uint8_t* kbase = p.k + hk * p.k_sh;
+  const uint8_t* vbase = p.v + hk * p.v_sh;
+
+  // this lane's offset from the first key its wavefront loads
+  const uint32_t k_off = (uint32_t)((lane / CH) * (int32_t)p.k_st + 16 * (lane % CH));
+  const uint32_t v_off = (uint32_t)((lane / CH) * (int32_t)p.v_st + 16 * (lane % CH));
+  // LDS byte offsets of this lane: K rows (A operand), V transposed reads
+  const int k_lane = lq * RP + 16 * k_slot<D>(lq, lh);
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int v_row = 4 * (g16 >> 1) + (s16 >> 2);
+  const int v_lane = K_BYTES + v_row * RP + 16 * v_slot<D>(v_row, 2 * (g16 & 1) + ((s16 & 3) >> 1)) + 8 * (s16 & 1);
+
+  for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
+    const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
+    const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
+    const int used = (tw.n + chunk - 1) / chunk;
+    if (z > 0 && z >= used) continue;  // part 0 writes the rows that see nothing
+    const int s0 = z * chunk, s1 = imin32(s0 + chunk, tw.n);
+
+    const int row = rt * ROWS + 32 * wave + lq;
+    const bool rok = row < n_rows;
+    const int t = rok ? udiv(row, p.div_g) : 0, h = hk * p.G + (rok ? row - t * p.G : 0);
+    const int ipos = sp.S - sp.n + t;
+    const RowKeys rk = rok ? cache_row_keys(p.mask, ipos, sp.S) : RowKeys{0, 0, 0};
+    float c1 = p.scale * (p.head_scale ? p.head_scale[h] : 1.f);
+    const float sl = p.alibi ? p.alibi[h] : 0.f;
+    if constexpr (SCORE == CACHE_SOFTMAX) c1 *= kCLog2e;
+    bf16x8_t qf[DK];
+    {
+      const uint16_t* qp = p.q + (int64_t)(sp.tok0 + t) * p.q_st + (int64_t)h * p.q_sh + 8 * here(lh);
+#pragma unroll
+      for (int kk = 0; kk < DK; ++kk) {
+        const u32x4_t w = *(const u32x4_t*)(qp + 16 * kk);
+        qf[kk] = __builtin_bit_cast(bf16x8_t, rok ? w : u32x4_t{0, 0, 0, 0});
+      }
+    }
+
+    // pages: numbers and scales of 64 from pg0 on, one per lane (every wavefront its own)
+    int32_t pg0 = 1 << 30, pg_id = -1;
+    float pg_ks = 0.f, pg_vs = 0.f;
+    auto pages_of = [&](int key) {
+      const int pg = key >> p.bshift, last = (key + BN - 16) >> p.bshift;
+      if (pg >= pg0 && last - pg0 <= 63) return;
+      pg0 = pg;
+      const int at = pg + here(lane);
+      pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
+      const int64_t id = imax32(pg_id, 0);
+      pg_ks = p.ks[id * p.ks_sb + hk * p.ks_sh];
+      pg_vs = p.vs[id * p.vs_sb + hk * p.vs_sh];
+    };
+    // what belongs to the four 16-key groups of a tile: of the one in the
+    // registers (next) and of the one in LDS that is computed (cur)
+    struct Groups {
+      int key;
+      float ks[4], vs[4];
+      bool full;  // every row of the workgroup's tile sees every key, every page is there
+      bool frac;  // some scale is no power of two
+      bool ok[4];
+    };
+    Groups next, cur;
+    cu32x4_t kr[NL], vr[NL];
+    auto load = [&](int s) {
+      next.key = walk_key(tw, s);
+      pages_of(next.key);
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        // chunk c of the tile: key c / CH; the 64 lanes of a wavefront stay inside one group of 16 keys
+        const int c0 = n * 256 + wave * 64, grp = c0 / CH / 16;
+        const int key = next.key + 16 * grp, id = __builtin_amdgcn_readlane(pg_id, (key >> p.bshift) - pg0);
+        const int64_t page = imax32(id, 0), place = (key & bs_mask) + (c0 / CH) % 16;
+        kr[n] = *(const cu32x4_t*)(kbase + page * p.k_sb + place * p.k_st + k_off);
+        vr[n] = *(const cu32x4_t*)(vbase + page * p.v_sb + place * p.v_st + v_off);
+      }
+    };
+    auto scales = [&]() {  // of the tile that load() has asked for
+      next.full = walk_full(tw, next.key, BN);
+      next.frac = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int at = ((next.key + 16 * q) >> p.bshift) - pg0;
+        next.ok[q] = __builtin_amdgcn_readlane(pg_id, at) >= 0;
+        next.ks[q] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_ks), at));
+        next.vs[q] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_vs), at));
+        next.full = next.full && next.ok[q];
+        next.frac = next.frac || fraction_of(next.ks[q]) != 1.f || fraction_of(next.vs[q]) != 1.f;
+      }
+    };
+    // The tile in the registers to LDS.  Where not every row sees every key, values
+    // that are no numbers are left out (0 x NaN must not reach the rows that do not
+    // see them) and noted; RAW, after the walk, stores them as they are.
+    auto store = [&](int stage, auto raw) __attribute__((always_inline)) {
+      constexpr bool RAW = decltype(raw)::value;
+      char* st = lds + stage * STAGE;
+      bool bad = false;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        const int c0 = n * 256 + wave * 64, grp = c0 / CH / 16;
+        const int row = (c0 / CH) + lane / CH, c = lane % CH;
+        const float ks = pow2_of(sel(grp >> 1, sel(grp & 1, next.ks[0], next.ks[1]), sel(grp & 1, next.ks[2], next.ks[3])));
+        const float vs = pow2_of(sel(grp >> 1, sel(grp & 1, next.vs[0], next.vs[1]), sel(grp & 1, next.vs[2], next.vs[3])));
+        cu32x4_t vw = vr[n];
+        if (!next.full) {
+          const bool there = next.key + row < sp.S && sel(grp >> 1, sel(grp & 1, next.ok[0], next.ok[1]), sel(grp & 1, next.ok[2], next.ok[3]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = there ? vr[n][i] : 0u, odd = vs < INFINITY ? nonfinite<FMT>(x) : 0x80808080u;
+            if constexpr (RAW) {
+              vw[i] = vs < INFINITY || !there ? x : 0x7f7f7f7fu;
+            } else {
+              vw[i] = x & ~((odd >> 7) * 0xffu);
+              bad = bad || (there && odd != 0);
+            }
+          }
+        }
+        if constexpr (!RAW) {
+          *(cu32x4_t*)(st + row * RP + 16 * k_slot<D>(row, 2 * c)) = cvt8<FMT>(kr[n][0], kr[n][1], ks);
+          *(cu32x4_t*)(st + row * RP + 16 * k_slot<D>(row, 2 * c + 1)) = cvt8<FMT>(kr[n][2], kr[n][3], ks);
+        }
+        const float f = RAW || !(next.full || vs < INFINITY) ? 1.f : vs;  // 0 times such a scale is no 0
+        *(cu32x4_t*)(st + K_BYTES + row * RP + 16 * v_slot<D>(row, 2 * c)) = cvt8<FMT>(vw[0], vw[1], f);
+        *(cu32x4_t*)(st + K_BYTES + row * RP + 16 * v_slot<D>(row, 2 * c + 1)) = cvt8<FMT>(vw[2], vw[3], f);
+      }
+      if (!RAW && !next.full && bad) poison_s = 1;
+    };
+    // bit e: the row sees key jb + 4 lh + 8 (e / 4) + e % 4
+    auto seen = [&](int jb, bool ok0, bool ok1) {
+      uint32_t vis = 0;
+      const int dres = p.mask.dil > 1 ? jb - udiv(jb, p.mask.div_dil) * p.mask.dil : 0;
+      const int ires = p.mask.dil > 1 && ipos >= 0 ? ipos - udiv(ipos, p.mask.div_dil) * p.mask.dil : 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = 4 * lh + 8 * (e >> 2) + (e & 3), j = jb + d;
+        bool ok = j >= rk.lo && j < rk.hi;
+        if (p.mask.dil > 1) {
+          const int jr = dres + d;
+          ok = ok && jr - udiv(jr, p.mask.div_dil) * p.mask.dil == ires;
+        }
+        ok = (ok || j < rk.pre) && (e < 8 ? ok0 : ok1);
+        vis |= (ok ? 1u : 0u) << e;
+      }
+      return vis;
+    };
+
+    f32x16_t acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[db][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+
+    // one 32-key block of the tile in LDS at `st`
+    auto block = [&](const char* st, int kb) __attribute__((always_inline)) {
+      const float ks2[2] = {sel(kb, cur.ks[0], cur.ks[2]), sel(kb, cur.ks[1], cur.ks[3])};
+      const float vs2[2] = {sel(kb, cur.vs[0], cur.vs[2]), sel(kb, cur.vs[1], cur.vs[3])};
+      const bool ok2[2] = {sel(kb, cur.ok[0], cur.ok[2]), sel(kb, cur.ok[1], cur.ok[3])};
+      const int jb = cur.key + 32 * kb;
+      const char* Kb = st + 32 * kb * RP;
+      f32x16_t s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+      __builtin_amdgcn_s_setprio(1);
+      bf16x8_t kf[DK];
+#pragma unroll
+      for (int kk = 0; kk < DK; ++kk) kf[kk] = *(const bf16x8_t*)(Kb + (k_lane ^ (32 * kk)));
+#pragma unroll
+      for (int kk = 0; kk < DK; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf[kk], s, 0, 0, 0);
+      // four LDS reads ahead of the MFMAs
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int kk = 4; kk < DK; ++kk) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      __builtin_amdgcn_s_setprio(0);
+      // V^T of the block's first 16 keys, on its way while the weights are made
+      bf16x8_t vf[2][DB];
+      auto read_v = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const char* pa = Kb + 16 * half * RP + (v_lane ^ (64 * db));
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)pa);
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP));
+          vf[half][db] = __builtin_bit_cast(bf16x8_t, (i16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      };
+      read_v(0);
+      __builtin_amdgcn_sched_barrier(0);
+      // key of register e: jb + 4 lh + 8 (e / 4) + e % 4; e < 8: the block's first group of 16
+      if (cur.frac)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= fraction_of(ks2[e >> 3]);
+      uint32_t vis = 0xffffu;
+      if (!cur.full) vis = seen(jb, ok2[0], ok2[1]);
+      asm("" : "+v"(vis));  // one register, not sixteen
+      if constexpr (SCORE != CACHE_SOFTMAX) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float v = __builtin_fmaf(sl, (float)(jb + 4 * lh + 8 * (e >> 2) + (e & 3) - ipos), s[e] * c1);
+          if (p.softcap > 0.f) {
+            const float ex = __builtin_amdgcn_exp2f(v * (2.f * kCLog2e / p.softcap));
+            v = p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + ex));
+          }
+          s[e] = SCORE == CACHE_SOFTMAX_MOD ? v * kCLog2e : v;
+        }
+      }
+      const float kq = SCORE == CACHE_SOFTMAX ? c1 : 1.f;  // s kq: the score in log2 units (softmax)
+      uint32_t pk[8];
+      if constexpr (SOFTMAX) {
+        if (!cur.full)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = (vis >> e) & 1 ? s[e] : -INFINITY;
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+        mx = xhalf_max(mx) * kq;
+        const float m_new = mx > m_run + kCLazy ? mx : m_run;
+        if (__any(m_new != m_run)) {
+          const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+          l_run *= a;
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[db][e] *= a;
+          m_run = m_new;
+        }
+        const float mo = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kq, mo));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float v = s[e];
+          if constexpr (SCORE == CACHE_SIGMOID)
+            v = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kCLog2e * (v + p.bias)));
+          else
+            v = v < 0.f ? 0.f : v;
+          s[e] = cur.full || ((vis >> e) & 1) ? v : 0.f;
+        }
+      }
+      float inv[2] = {1.f, 1.f};
+      if (cur.frac) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float f = fraction_of(vs2[q]);
+          inv[q] = 1.f / f;
+#pragma unroll
+          for (int e = 8 * q; e < 8 * q + 8; ++e) s[e] = (vis >> e) & 1 ? s[e] * f : 0.f;
+        }
+      }
+      float ls[2] = {0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const bf16x2_t pb = pack2(s[2 * w], s[2 * w + 1]);
+        if constexpr (SOFTMAX) ls[w >> 2] = __builtin_amdgcn_fdot2_f32_bf16(pb, kOnes2, ls[w >> 2], false);
+        pk[w] = __builtin_bit_cast(uint32_t, pb);
+      }
+      if constexpr (SOFTMAX) l_run = __builtin_fmaf(ls[0], inv[0], __builtin_fmaf(ls[1], inv[1], l_run));
+
+      read_v(1);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, u32x4_t{pk[4 * half], pk[4 * half + 1], pk[4 * half + 2], pk[4 * half + 3]});
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[half][db], pf, acc[db], 0, 0, 0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+    };
+
+    if (s0 < s1) {
+      __syncthreads();  // the tile before has been looked at
+      if (tid == 0) poison_s = 0;
+      load(s0);
+      scales();
+      __syncthreads();
+      store(0, BoolTag<false>());
+      __syncthreads();
+      for (int s = s0; s < s1; ++s) {
+        cur = next;
+        const bool more = s + 1 < s1;
+        if (more) load(s + 1);
+        const int stage = (s - s0) & 1;
+#pragma unroll 1
+        for (int kb = 0; kb < 2; ++kb) block(lds + stage * STAGE, kb);
+        if (more) {
+          scales();
+          store(stage ^ 1, BoolTag<false>());
+        }
+        __syncthreads();
+      }
+      if (poison_s != 0) {
+        // The rows that see a value that is no number: its NaN, or its infinity (NaN for
+        // ReLU, whose weight may be 0), by products of 1 at such values with 1 at the
+        // keys that a row sees.
+        for (int s = s0; s < s1; ++s) {
+          load(s);
+          scales();
+          if (next.full) continue;
+          __syncthreads();
+          store(0, BoolTag<true>());
+          __syncthreads();
+#pragma unroll 1
+          for (int hb = 0; hb < 4; ++hb) {
+            const uint32_t vis = seen(next.key + 32 * (hb >> 1), sel(hb >> 1, next.ok[0], next.ok[2]), sel(hb >> 1, next.ok[1], next.ok[3])) >> (8 * (hb & 1));
+            u32x4_t sees;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sees[i] = ((vis >> (2 * i)) & 1 ? 0x3f80u : 0u) | ((vis >> (2 * i + 1)) & 1 ? 0x3f800000u : 0u);
+            const bf16x8_t sf = __builtin_bit_cast(bf16x8_t, sees);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              const char* pa = lds + 16 * hb * RP + (v_lane ^ (64 * db));
+              const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)pa);
+              const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP));
+              const i16x8_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+              i16x8_t nan, up, down;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int m = a[i] & 0x7fff;
+                const bool inf = SCORE != CACHE_RELU && m == 0x7f80;
+                nan[i] = m >= 0x7f80 && !inf ? (short)0x3f80 : (short)0;
+                up[i] = inf && a[i] >= 0 ? (short)0x3f80 : (short)0;
+                down[i] = inf && a[i] < 0 ? (short)0x3f80 : (short)0;
+              }
+              f32x16_t zero;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+              const f32x16_t n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, nan), sf, zero, 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[db][e] = n[e] > 0.f ? NAN : acc[db][e];
+              if constexpr (FMT == 1) {
+                const f32x16_t u = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, up), sf, zero, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[db][e] += u[e] > 0.f ? INFINITY : 0.f;
+                const f32x16_t v = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, down), sf, zero, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[db][e] -= v[e] > 0.f ? INFINITY : 0.f;
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
+    }
+
+    if constexpr (SOFTMAX) l_run = xhalf_sum(l_run);
+    if (rok) {
+      if (used <= 1) {
+        const float f = SOFTMAX ? (l_run != 0.f ? 1.f / l_run : 0.f) : p.post_scale;
+        uint16_t* op = p.o + (int64_t)(sp.tok0 + t) * p.o_st + (int64_t)h * p.o_sh + 4 * here(lh);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *(u32x2_t*)(op + 32 * db + 8 * q) = u32x2_t{pack_bf16x2(acc[db][4 * q] * f, acc[db][4 * q + 1] * f),
+                                                       pack_bf16x2(acc[db][4 * q + 2] * f, acc[db][4 * q + 3] * f)};
+      } else {
+        const int64_t at = ((int64_t)z * p.T + sp.tok0 + t) * p.H + h;
+        float* op = p.part_o + at * D + 4 * here(lh);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *(f32x4_t*)(op + 32 * db + 8 * q) = f32x4_t{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2], acc[db][4 * q + 3]};
+        if (SOFTMAX && lh == 0) {
+          p.part_ml[2 * at] = m_run;
+          p.part_ml[2 * at + 1] = l_run;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace chia

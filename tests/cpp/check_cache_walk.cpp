@@ -40,14 +40,15 @@ int main() {
     const int S = rnd(10) ? rnd(400) : rnd(3);
     const int n = 1 + rnd(40), i0 = S - n + rnd(n), i1 = i0 + rnd(S - i0 > 0 ? S - i0 : 1);
     if (i1 >= S && S > 0) continue;
-    const TileWalk w = cache_tile_walk(m, i0, i1, S);
+    const int kStepKeys = rnd(2) ? 32 : 64;
+    const TileWalk w = cache_tile_walk(m, i0, i1, S, kStepKeys);
     std::vector<int> times(S + 64, 0);
     for (int s = 0; s < w.n; ++s) {
       const int c = walk_key(w, s);
       if (c < 0 || c % kStepKeys || c >= S + kStepKeys) ++failures;
       for (int x = 0; x < kStepKeys; ++x)
         if (c + x < S + 64) ++times[c + x];
-      for (int len : {16, 32}) {
+      for (int len : {16, 32, 64}) {
         bool all = true;
         for (int i = i0; i <= i1; ++i)
           for (int x = 0; x < len; ++x) all = all && sees(m, i, c + x, S);
@@ -73,7 +74,7 @@ int main() {
   }
   // causal walks skip what lies behind: a decoding step under a window reads only the window
   CacheMask m{1, 64, 1, 0, 0, make_udiv(1), make_udiv(1)};
-  if (cache_tile_walk(m, 9999, 9999, 10000).n > 3) ++failures;
+  if (cache_tile_walk(m, 9999, 9999, 10000, 32).n > 3) ++failures;
   // far positions and reaches do not overflow
   const int big = (1 << 28) - 1;
   CacheMask f{0, big, 1, big, 1 << 28, make_udiv(big), make_udiv(1)};
