@@ -92,33 +92,45 @@ def extend_block_tables(block_tables: torch.Tensor, context_lens: torch.Tensor, 
     if torch.compiler.is_compiling():
         return CacheStep(*torch.ops.chia_attn.extend_block_tables(block_tables, context_lens, new_lens, free_blocks,
                                                                   free_count, block_size, max_tokens))
-    device = _check_table(block_tables, block_size)
-    R = block_tables.shape[0]
-    for name, t, n in (("context_lens", context_lens, R), ("new_lens", new_lens, R), ("free_blocks", free_blocks, None),
-                       ("free_count", free_count, 1)):
-        _contiguous(name, _vector(name, t, device, (n,)))
-    if max_tokens < 0:
-        raise ValueError(f"max_tokens must be >= 0, got {max_tokens}")
-    T = int(max_tokens)
+    # as in attention(): a call with the shapes and layouts of an earlier one reuses
+    # its validated argument struct; only the pointers are new
+    try:
+        key = ("cache_tables", block_size, max_tokens) + _meta(block_tables, context_lens, new_lens, free_blocks,
+                                                               free_count)
+        cache = _args_cache()
+        entry = cache.get(key)
+    except (AttributeError, TypeError):
+        entry = key = None
+    if entry is None:
+        device = _check_table(block_tables, block_size)
+        R = block_tables.shape[0]
+        for name, t, n in (("context_lens", context_lens, R), ("new_lens", new_lens, R),
+                           ("free_blocks", free_blocks, None), ("free_count", free_count, 1)):
+            _contiguous(name, _vector(name, t, device, (n,)))
+        if max_tokens < 0:
+            raise ValueError(f"max_tokens must be >= 0, got {max_tokens}")
+        T = int(max_tokens)
+        a = _lib.CacheTablesArgs(block_size=block_size, table_stride=_row_stride(block_tables), requests=R,
+                                 width=block_tables.shape[1], free_capacity=free_blocks.shape[0], max_tokens=T)
+        entry = (a, device, T, R, (T, T, R + 1, R, 1, 1))
+        if key is not None and R > 0:
+            _remember(cache, key, entry)
+    a, device, T, R, sizes = entry
     # one allocation: slots, positions, offsets, lengths, the two counts
     flat = torch.empty(2 * T + 2 * R + 3, dtype=torch.int32, device=device)
-    step = CacheStep(*flat.split((T, T, R + 1, R, 1, 1)))
+    step = CacheStep._make(flat.split_with_sizes(sizes))
     if R == 0:
         flat.fill_(-1)
         step.cu_seqlens.zero_()
         step.missing.zero_()
         step.free_count.copy_(free_count.clamp(0, free_blocks.shape[0]))
         return step
-    a = _lib.CacheTablesArgs(block_size=block_size, block_tables=block_tables.data_ptr(),
-                             table_stride=_row_stride(block_tables), requests=R, width=block_tables.shape[1],
-                             context_lens=context_lens.data_ptr(), new_lens=new_lens.data_ptr(),
-                             free_blocks=free_blocks.data_ptr(), free_count=free_count.data_ptr(),
-                             free_capacity=free_blocks.shape[0], max_tokens=T)
     at = flat.data_ptr()
+    a.block_tables, a.context_lens, a.new_lens = block_tables.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr()
+    a.free_blocks, a.free_count = free_blocks.data_ptr(), free_count.data_ptr()
     a.slots, a.positions, a.cu_seqlens = at, at + 4 * T, at + 8 * T
-    a.seq_lens = a.cu_seqlens + 4 * (R + 1)
-    a.free_left = a.seq_lens + 4 * R
-    a.missing = a.free_left + 4
+    at += 8 * T + 4 * (R + 1)
+    a.seq_lens, a.free_left, a.missing = at, at + 4 * R, at + 4 * R + 4
     with _device_of(block_tables):
         _lib.cache_tables(a, _current_stream(block_tables))
     return step
@@ -180,7 +192,8 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale):
 
 
 def _meta(*tensors):
-    return tuple((t.shape, t.dtype, t.device, t.stride()) for t in tensors)
+    """What a cached call is recognised by: shapes, types, devices and layouts."""
+    return tuple([(t.shape, t.dtype, t.device, t.stride()) for t in tensors])
 
 
 def _laid_out(t: torch.Tensor) -> torch.Tensor:
@@ -274,16 +287,15 @@ def attention_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     queries and tokens; they size the launch, and exceeding them costs time, not
     results.  Returns o bf16 [T, H, D].  Forward only.
     """
-    params = dict(norm=norm, causal=causal, window=window, dilation=dilation, block=block, prefix=prefix, scale=scale,
-                  head_scale=head_scale, alibi_slopes=alibi_slopes, softcap=softcap, bias=bias, post_scale=post_scale)
-    if torch.is_grad_enabled() and isinstance(q, torch.Tensor) and q.requires_grad:
+    if isinstance(q, torch.Tensor) and q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention_cache is forward only: q must not require grad")
     if torch.compiler.is_compiling():
         if out is not None:
             raise ValueError("out= is not supported under torch.compile")
         from .library import call_cache_attn
 
-        p = dict(params)
+        p = dict(norm=norm, causal=causal, window=window, dilation=dilation, block=block, prefix=prefix, scale=scale,
+                 head_scale=head_scale, alibi_slopes=alibi_slopes, softcap=softcap, bias=bias, post_scale=post_scale)
         for name, positive in (("head_scale", True), ("alibi_slopes", False)):
             p[name] = _per_head_vector(p[name], q.shape[1], q.device, name, positive=positive, cache=False)
         return call_cache_attn(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_seqlens, max_query,

@@ -130,7 +130,13 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   const int64_t most = !t->cu_seqlens ? 1 : a->max_query < a->queries ? a->max_query : a->queries;
   const int64_t rows = G * (most < 1 ? 1 : most);
   Shape s;
-  s.tile = rows <= 16 ? CACHE_ROWS16 : rows <= 32 ? CACHE_ROWS32 : CACHE_ROWS128;
+  // 32 rows to a workgroup start and split better, 128 compute faster: about 870 and
+  // 1700 (row x key)s per ns on a full chip, and 17 us more for the latter's longer steps
+  // (H32/8 D128, us with 32 and 128: one prompt of 300 tokens 17, 29; 8 of 48 over 4000: 70, 68;
+  // 32 of 32 over 4000: 134, 119; 64 of 10 over 4000, whose 40 rows fill 64 and 128: 145, 186).
+  const double each = (double)(t->batch * hkv) * (double)(t->seqlen < a->width * a->block_size ? t->seqlen : a->width * a->block_size);
+  const double us32 = each * (double)((rows + 31) / 32 * 32) / 0.87e6, us128 = each * (double)((rows + 127) / 128 * 128) / 1.7e6 + 17.0;
+  s.tile = rows <= 16 ? CACHE_ROWS16 : us32 <= us128 ? CACHE_ROWS32 : CACHE_ROWS128;
   const int R = kCacheRows[s.tile];
   s.tiles = (rows + R - 1) / R;
   // steps of the longest request's last tile
@@ -142,26 +148,36 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   const int64_t groups = t->batch * hkv * s.tiles;
   // How many parts.  A part costs a workgroup's start and end (lengths, table, first
   // keys; merge) whatever it holds, the second kernel 3 to 5 us, and too few parts
-  // leave CUs idle or waiting for the longest request.  With `room` the workgroups
-  // that the chip holds at once:
-  //   * 16-row tiles, up to 128 (request, head) pairs: 3/4 of room, since their parts
-  //     are nearly equal (2 requests of 131072 tokens, H32/8 D128, us by workgroups asked for:
-  //     100 (512), 103 (768), 109 (1024); 11 of up to 32318, H16/8 D64: 90, 68, 70); beyond,
-  //     3/2 of it, since many of their parts do not exist (16 of 33 .. 4096, 16 heads, D64: 38 (512), 33 (1024),
-  //     28 (1536), 33 (2048));
-  //   * two workgroups per CU: room (16 requests verifying 5 tokens over 4096, H32/8 D128: 35 (512), 42, 47);
-  //   * parts of 16 steps (512 keys) or more, of 8 where that is a handful of workgroups
-  //     (2 of 2994, 2 heads: 13.1 -> 11.6);
-  //   * but, for balance, no parts much beyond 48 steps (64 of 97 .. 8192, H32/8 D128: 125 (1 part),
-  //     113 (4), 106 (5), 108 (6)).
+  // leave CUs idle or waiting for the longest request.  us by workgroups asked for: 2
+  // requests of 131072 tokens, H32/8 D128, 100 (512), 118 (576), 103 (768), 109 (1024); 11 of up to 32318,
+  // H16/8 D64, 90 (440), 68 (704), 77 (1496); 16 of 33 .. 4096, 16 heads, D64, 38 (512), 33 (1024), 28 (1536),
+  // 33 (2048); 64 of 97 .. 8192, H32/8 D128, 125 (1 part), 113 (4), 106 (5), 108 (6); 16 verifying 5 tokens over 4096,
+  // 35 (512), 42 (768), 47 (1024); 2 of 2994, 2 heads, parts of 16 steps 13.1, of 8 11.6.
   const bool small = s.tile == CACHE_ROWS16;
-  const int64_t room = kCUs * (small ? (t->head_dim == 64 ? 4 : 3) : 2);
-  const int64_t least = groups * steps <= 2048 && steps > 32 && small ? 8 : 16;
-  int64_t parts = (!small ? room : groups <= 128 ? room * 3 / 4 : room * 3 / 2) / groups;
+  const int64_t most_wgs = small ? (t->head_dim == 64 ? 4 : 3) : 2;  // per CU at once
+  int64_t least = 16, parts;
+  if (s.tile == CACHE_ROWS128) least = 4;
+  else if (small && groups * steps <= 2048 && steps > 32) least = 8;
+  if (groups <= 128 || !small) {
+    // Few (request, head, row tile)s: their parts are nearly equal, so that the CUs with
+    // most of them set the time: the number whose 2, 3 or 4 per CU leave the fewest
+    // places empty.
+    parts = 1;
+    double best = 0.0;
+    for (int64_t k = 2; k <= most_wgs; ++k) {
+      const int64_t n = k * kCUs / groups;
+      const double used = (double)(n * groups) / (double)(k * kCUs);
+      if (n >= 1 && used > best + 0.02) best = used, parts = n;
+    }
+  } else {
+    // Many: their parts are of unequal length or not there at all, and half as many
+    // again as the chip holds keep it full; but, for balance, no parts much beyond 48 steps.
+    parts = most_wgs * kCUs * 3 / 2 / groups;
+    int64_t balance = steps / 48;
+    if (balance > 6 * most_wgs * kCUs / groups) balance = 6 * most_wgs * kCUs / groups;
+    if (parts < balance) parts = balance;
+  }
   if (parts > steps / least) parts = steps / least;
-  int64_t balance = steps / 48;
-  if (balance > 6 * room / groups) balance = 6 * room / groups;
-  if (s.tile != CACHE_ROWS128 && parts < balance && groups > 128) parts = balance;
   if (parts < 1) parts = 1;
   s.chunk = (steps + parts - 1) / parts;
   s.parts = (steps + s.chunk - 1) / s.chunk;

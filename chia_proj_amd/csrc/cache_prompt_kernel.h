@@ -67,14 +67,22 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
   const uint8_t* kbase = p.k + hk * p.k_sh;
   const uint8_t* vbase = p.v + hk * p.v_sh;
 
-  // this lane's offset from the first key its wavefront loads
-  const uint32_t k_off = (uint32_t)((lane / CH) * (int32_t)p.k_st + 16 * (lane % CH));
-  const uint32_t v_off = (uint32_t)((lane / CH) * (int32_t)p.v_st + 16 * (lane % CH));
+  // This lane's key among the 8 (D = 128) or 16 that its wavefront loads together, its
+  // 16 codes of it, and its offset from the first.  Four lanes take 64 bytes of a key, the
+  // next four those of the key whose swizzle differs in the lowest bit: a lane's codes
+  // become an even and an odd 16-byte piece, and eight lanes' even pieces then lie in
+  // eight different slots.
+  const int q = lane >> 2, in_row = D == 128 ? (q >> 2) | ((q & 1) << 2) : (q >> 1) | ((q & 1) << 3);
+  const int in_c = D == 128 ? (lane & 3) | ((q & 2) << 1) : lane & 3;
+  const uint32_t k_off = (uint32_t)(in_row * (int32_t)p.k_st + 16 * in_c);
+  const uint32_t v_off = (uint32_t)(in_row * (int32_t)p.v_st + 16 * in_c);
   // LDS byte offsets of this lane: K rows (A operand), V transposed reads
   const int k_lane = lq * RP + 16 * k_slot<D>(lq, lh);
   const int g16 = lane >> 4, s16 = lane & 15;
   const int v_row = 4 * (g16 >> 1) + (s16 >> 2);
-  const int v_lane = K_BYTES + v_row * RP + 16 * v_slot<D>(v_row, 2 * (g16 & 1) + ((s16 & 3) >> 1)) + 8 * (s16 & 1);
+  const int v_lane = K_BYTES + v_row * RP + 16 * k_slot<D>(v_row, 2 * (g16 & 1) + ((s16 & 3) >> 1)) + 8 * (s16 & 1);
+
+  constexpr int SW8 = D == 128 ? 32 : 16;  // 16 row_swz(8): rows 8 further on flip this bit of the slot
 
   for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
     const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
@@ -140,6 +148,17 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
     };
     auto scales = [&]() {  // of the tile that load() has asked for
       next.full = walk_full(tw, next.key, BN);
+      if (p.bshift >= 6) {  // one page
+        const int at = (next.key >> p.bshift) - pg0;
+        const bool ok = __builtin_amdgcn_readlane(pg_id, at) >= 0;
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_ks), at));
+        const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pg_vs), at));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) next.ok[q] = ok, next.ks[q] = ks, next.vs[q] = vs;
+        next.full = next.full && ok;
+        next.frac = fraction_of(ks) != 1.f || fraction_of(vs) != 1.f;
+        return;
+      }
       next.frac = false;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -161,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
 #pragma unroll
       for (int n = 0; n < NL; ++n) {
         const int c0 = n * 256 + wave * 64, grp = c0 / CH / 16;
-        const int row = (c0 / CH) + lane / CH, c = lane % CH;
+        const int row = (c0 / CH) + in_row, c = in_c;
         const float ks = pow2_of(sel(grp >> 1, sel(grp & 1, next.ks[0], next.ks[1]), sel(grp & 1, next.ks[2], next.ks[3])));
         const float vs = pow2_of(sel(grp >> 1, sel(grp & 1, next.vs[0], next.vs[1]), sel(grp & 1, next.vs[2], next.vs[3])));
         cu32x4_t vw = vr[n];
@@ -178,13 +197,15 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
             }
           }
         }
-        if constexpr (!RAW) {
-          *(cu32x4_t*)(st + row * RP + 16 * k_slot<D>(row, 2 * c)) = cvt8<FMT>(kr[n][0], kr[n][1], ks);
-          *(cu32x4_t*)(st + row * RP + 16 * k_slot<D>(row, 2 * c + 1)) = cvt8<FMT>(kr[n][2], kr[n][3], ks);
-        }
         const float f = RAW || !(next.full || vs < INFINITY) ? 1.f : vs;  // 0 times such a scale is no 0
-        *(cu32x4_t*)(st + K_BYTES + row * RP + 16 * v_slot<D>(row, 2 * c)) = cvt8<FMT>(vw[0], vw[1], f);
-        *(cu32x4_t*)(st + K_BYTES + row * RP + 16 * v_slot<D>(row, 2 * c + 1)) = cvt8<FMT>(vw[2], vw[3], f);
+        char* at = st + row * RP;
+        const int slot0 = 16 * k_slot<D>(row, 2 * c), slot1 = 16 * k_slot<D>(row, 2 * c + 1);
+        if constexpr (!RAW) {
+          *(cu32x4_t*)(at + slot0) = cvt8<FMT>(kr[n][0], kr[n][1], ks);
+          *(cu32x4_t*)(at + slot1) = cvt8<FMT>(kr[n][2], kr[n][3], ks);
+        }
+        *(cu32x4_t*)(at + K_BYTES + slot0) = cvt8<FMT>(vw[0], vw[1], f);
+        *(cu32x4_t*)(at + K_BYTES + slot1) = cvt8<FMT>(vw[2], vw[3], f);
       }
       if (!RAW && !next.full && bad) poison_s = 1;
     };
@@ -244,9 +265,9 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
       auto read_v = [&](int half) __attribute__((always_inline)) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const char* pa = Kb + 16 * half * RP + (v_lane ^ (64 * db));
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)pa);
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP));
+          const char* pa = Kb + 16 * half * RP;
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (v_lane ^ (64 * db))));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (v_lane ^ (64 * db) ^ SW8)));
           vf[half][db] = __builtin_bit_cast(bf16x8_t, (i16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
       };
@@ -377,9 +398,9 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
             const bf16x8_t sf = __builtin_bit_cast(bf16x8_t, sees);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-              const char* pa = lds + 16 * hb * RP + (v_lane ^ (64 * db));
-              const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)pa);
-              const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP));
+              const char* pa = lds + 16 * hb * RP;
+              const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (v_lane ^ (64 * db))));
+              const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (v_lane ^ (64 * db) ^ SW8)));
               const i16x8_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
               i16x8_t nan, up, down;
 #pragma unroll

@@ -40,6 +40,9 @@ struct WriteParams {
   UDiv div_h;
 };
 
+// A scale that was there; 0 for what is none.
+__device__ __forceinline__ float usable(float s) { return s > 0.f && s < INFINITY ? s : 0.f; }
+
 template <int FMT>  // CHIA_ATTN_FP8_E4M3 / E5M2
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   int r;
@@ -107,6 +110,43 @@ __device__ __forceinline__ float need_of(uint32_t bits) {
   return __uint_as_float((uint32_t)((e < -126 ? -126 : e) + 127) << 23);
 }
 
+// Eight bf16 values to codes.
+template <int FMT>
+__device__ __forceinline__ u32x2_t codes_of(u32x4_t x, float scale, float inv, bool pow2) {
+  float f[8];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[2 * w] = bounded<FMT>(over(__uint_as_float(x[w] << 16), scale, inv, pow2));
+    f[2 * w + 1] = bounded<FMT>(over(__uint_as_float(x[w] & 0xffff0000u), scale, inv, pow2));
+  }
+  return u32x2_t{pack4<FMT>(f[0], f[1], f[2], f[3]), pack4<FMT>(f[4], f[5], f[6], f[7])};
+}
+
+// The first `rows` rows of a page to a scale that has grown: chunks first, first + step, ...
+template <int D, int FMT>
+__device__ __forceinline__ void rescale(uint8_t* page, int64_t row_stride, int rows, float ratio, int first, int step) {
+  constexpr int LPR = D / 8;
+  for (int c = first; c < rows * LPR; c += step) {
+    u32x2_t* at = (u32x2_t*)(page + (int64_t)(c / LPR) * row_stride + (c % LPR) * 8);
+    u32x2_t v = *at;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      v[w] = pack4<FMT>(bounded<FMT>(times(code_at<FMT>(v[w], 0), ratio)), bounded<FMT>(times(code_at<FMT>(v[w], 1), ratio)),
+                        bounded<FMT>(times(code_at<FMT>(v[w], 2), ratio)), bounded<FMT>(times(code_at<FMT>(v[w], 3), ratio)));
+    *at = v;
+  }
+}
+
+__device__ __forceinline__ uint32_t largest(u32x4_t x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t lo = finite_bits(x[w]), hi = finite_bits(x[w] >> 16), h = lo > hi ? lo : hi;
+    m = m > h ? m : h;
+  }
+  return m;
+}
+
 // W wavefronts to a team; N 16-byte chunks of a run per lane.
 template <int D, int FMT, int W, int N>
 __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
@@ -133,9 +173,58 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
   for (int base = t0; base < t0 + p.window; base += 64) {
     // the runs that begin at tokens base .. base + 63 of this window
     const int t = base + lane;
-    const int32_t mine = t < t_end ? slot_at(t) : -1;
-    const int32_t before = t < t_end ? slot_at(t - 1) : -1;
-    uint64_t starts = __ballot(mine >= 0 && (before < 0 || before + 1 != mine || (mine & (bs - 1)) == 0));
+    const int32_t mine = slot_at(t), before = slot_at(t - 1);
+    const bool begins = mine >= 0 && (before < 0 || before + 1 != mine || (mine & (bs - 1)) == 0);
+    uint64_t starts = __ballot(begins && t < t_end);
+    const uint64_t goes_on = __ballot(mine >= 0 && !begins);  // continues the run of the token before
+    // Runs of one token (decoding requests among prompts): a row's lanes to each,
+    // several at a time, rather than the whole team to one after the other.
+    const uint64_t single = starts & ~(goes_on >> 1) & ~(1ull << 63);
+    if (single) {
+      constexpr int PER = 64 / LPR, DEEP = 4;  // tokens at a time, rounds in flight
+      const int count = __popcll(single);
+      starts &= ~single;
+      // lane i: the token of the i-th of them
+      const bool is = (single >> lane) & 1;
+      const int rank = __popcll(single & ((1ull << lane) - 1));
+      const int order = __builtin_amdgcn_ds_permute((is ? rank : count + lane - rank) << 2, lane);
+      for (int k0 = (wave % W) * DEEP * PER; k0 < count; k0 += W * DEEP * PER) {
+        u32x4_t x[DEEP];
+        int32_t slot[DEEP];
+        float old[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+          const int i = k0 + k * PER + lane / LPR, at = __shfl(order, i & 63);
+          const int32_t v = __shfl(mine, at);
+          slot[k] = i < count ? v : -1;
+          x[k] = u32x4_t{0, 0, 0, 0};
+          old[k] = 0.f;
+          if (slot[k] >= 0) {
+            x[k] = *(const u32x4_t*)(s.x + (int64_t)(base + at) * s.x_st + head * s.x_sh + (lane % LPR) * 8);
+            if (slot[k] & (bs - 1)) old[k] = s.scale[(int64_t)(slot[k] >> p.bshift) * s.s_sb + head * s.s_sh];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+          uint32_t amax = largest(x[k]);
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_xor((int)amax, d);
+            amax = amax > o ? amax : o;
+          }
+          if (slot[k] < 0) continue;
+          const int off = slot[k] & (bs - 1);
+          const int64_t page = slot[k] >> p.bshift;
+          old[k] = usable(old[k]);
+          const float need = need_of<FMT>(amax), scale = need > old[k] ? need : old[k];
+          const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0, grown = off > 0 && scale != old[k];
+          if (lane % LPR == 0 && (off == 0 || grown)) s.scale[page * s.s_sb + head * s.s_sh] = scale;
+          uint8_t* cp = s.codes + page * s.c_sb + head * s.c_sh;
+          *(u32x2_t*)(cp + (int64_t)off * s.c_st + (lane % LPR) * 8) = codes_of<FMT>(x[k], scale, 1.f / scale, pow2);
+          if (grown) rescale<D, FMT>(cp, s.c_st, off, old[k] / scale, lane % LPR, LPR);
+        }
+      }
+    }
     while (true) {
       bool any = starts != 0;
       if constexpr (W == 2) {
@@ -150,13 +239,18 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
       const int off = slot & (bs - 1);
       int len = 0;  // tokens of the run
       if (live) {
-        const int most = bs - off;
-        while (len < most) {
-          const int k = len + lane;
-          const uint64_t same = __ballot(k < most && slot_at(run_t + k) == slot + k);
-          const int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
-          len += n;
-          if (n < 64) break;
+        const uint64_t behind = i < 63 ? ~(goes_on >> (i + 1)) : ~0ull;  // its lowest bit: the first that does not go on
+        len = i < 63 ? 1 + __builtin_ctzll(behind) : 1;
+        if (len > 63 - i) {  // up to the last lane, and perhaps further
+          len = 64 - i;
+          const int most = bs - off;
+          while (len < most) {
+            const int k = len + lane;
+            const uint64_t same = __ballot(k < most && slot_at(run_t + k) == slot + k);
+            const int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
+            len += n;
+            if (n < 64) break;
+          }
         }
       }
       const int64_t page = slot >> p.bshift;
@@ -172,13 +266,10 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
         if (row < len) x[n] = *(const u32x4_t*)(xr + (int64_t)row * s.x_st + col * 8);
       }
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t lo = finite_bits(x[n][w]), hi = finite_bits(x[n][w] >> 16);
-          const uint32_t m = lo > hi ? lo : hi;
-          amax = amax > m ? amax : m;
-        }
+      for (int n = 0; n < N; ++n) {
+        const uint32_t m = largest(x[n]);
+        amax = amax > m ? amax : m;
+      }
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const uint32_t o = (uint32_t)__shfl_xor((int)amax, d);
@@ -195,7 +286,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
         __syncthreads();
       }
       if (live) {
-        if (!(old > 0.f) || old > 3.0e38f) old = 0.f;
+        old = usable(old);
         const float need = need_of<FMT>(amax);
         const float scale = need > old ? need : old;
         const bool grown = off > 0 && scale != old;
@@ -206,30 +297,10 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
           const int c = n * (64 * W) + tl, row = c / LPR, col = c % LPR;
-          if (row < len) {
-            float f[8];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const float a = __uint_as_float(x[n][w] << 16), b = __uint_as_float(x[n][w] & 0xffff0000u);
-              f[2 * w] = bounded<FMT>(over(a, scale, inv, pow2));
-              f[2 * w + 1] = bounded<FMT>(over(b, scale, inv, pow2));
-            }
-            *(u32x2_t*)(cp + (int64_t)(off + row) * s.c_st + col * 8) =
-                u32x2_t{pack4<FMT>(f[0], f[1], f[2], f[3]), pack4<FMT>(f[4], f[5], f[6], f[7])};
-          }
+          if (row < len)
+            *(u32x2_t*)(cp + (int64_t)(off + row) * s.c_st + col * 8) = codes_of<FMT>(x[n], scale, inv, pow2);
         }
-        if (grown) {  // the codes from before, to the new scale
-          const float ratio = old / scale;
-          for (int c = tl; c < off * LPR; c += 64 * W) {
-            u32x2_t* at = (u32x2_t*)(cp + (int64_t)(c / LPR) * s.c_st + (c % LPR) * 8);
-            u32x2_t v = *at;
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-              v[w] = pack4<FMT>(bounded<FMT>(times(code_at<FMT>(v[w], 0), ratio)), bounded<FMT>(times(code_at<FMT>(v[w], 1), ratio)),
-                                bounded<FMT>(times(code_at<FMT>(v[w], 2), ratio)), bounded<FMT>(times(code_at<FMT>(v[w], 3), ratio)));
-            *at = v;
-          }
-        }
+        if (grown) rescale<D, FMT>(cp, s.c_st, off, old / scale, tl, 64 * W);
         starts &= starts - 1;
       }
     }
@@ -300,12 +371,15 @@ extern "C" int chia_cache_write(const chia_cache_write_args* a, void* stream) {
   const WriteKernel k = a->head_dim == 64 ? (fmt ? pick<64, 1>(bs) : pick<64, 0>(bs))
                                           : (fmt ? pick<128, 1>(bs) : pick<128, 0>(bs));
   if (!k.fn) return CHIA_ATTN_ERR_SHAPE;
-  // A window of tokens per team: one where every token may begin a run of its own
-  // and there are teams to spare, more (up to a page) where that many teams would
-  // mostly find that their token continues a run.
+  // A window of tokens per team: as many as a wavefront has rows' worth of lanes (4 or
+  // 8), since each may be a run of its own (decoding), and more, up to a page, where
+  // that many teams would mostly find that their tokens continue a run (prompts): as many as keep 2048 teams (8 thousand tokens of
+  // 16 heads, D = 64, pages of 64: 33 us with 65536 teams, 24 with 16384, 16 with 4096; 16384 of 8,
+  // D = 128, pages of 128: 37 with 4096, 25 with 2048).
   int64_t units = 2 * a->kv_heads * a->tokens;
-  p.window = 1;
-  while (p.window < bs && units > 65536) {
+  p.window = 512 / (int)a->head_dim;
+  units = 2 * a->kv_heads * ((a->tokens + p.window - 1) / p.window);
+  while (p.window < bs && units > 2048) {
     p.window *= 2;
     units = 2 * a->kv_heads * ((a->tokens + p.window - 1) / p.window);
   }

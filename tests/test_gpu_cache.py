@@ -231,7 +231,7 @@ def test_write_many_tokens_in_windows():
     slots = [p * bs + i for p in order[:500] for i in range(bs)][3:]
     slots += [p * bs + int(torch.randint(0, bs, (1,), generator=g)) for p in order[500:]]
     k = torch.randn(len(slots), H, D, generator=g).to(torch.bfloat16)
-    assert 2 * H * len(slots) > 65536
+    assert 2 * H * len(slots) > 65536  # several tokens to a team
     _check_write(k, k * 3, kc, kc.clone(), ks, ks.clone(), slots)
 
 
