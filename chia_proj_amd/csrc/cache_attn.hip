@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnParams 
   const int slot = (int)threadIdx.x / LPR, d = 4 * ((int)threadIdx.x % LPR), zi = slot % ZG;
   const int64_t th = (int64_t)p.T * p.H;
   for (int rt = rt0; rt * ROWS + sub * RPW < n_rows; rt += p.tiles) {
-    const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
+    const TileWalk tw = cache_walk_of<ROWS>(p.mask, p.div_g, sp, rt);
     const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
     const int used = (tw.n + chunk - 1) / chunk;
     if (used <= 1) continue;

@@ -66,6 +66,16 @@ struct CacheAttnParams {
 constexpr float kCLog2e = 1.4426950408889634f;
 constexpr float kCLazy = 8.0f;
 
+// The kernel's arguments where they are used seldom (a page lookup, a masked step,
+// the end): read again from the argument segment there, rather than held in scalar
+// registers, and spilled, through the walk.
+using ColdArgs = const __attribute__((address_space(4))) CacheAttnParams*;
+__device__ __forceinline__ ColdArgs cold_args() {
+  ColdArgs p = (ColdArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 // What a workgroup computes for one (request, K/V head): the request's span.
 struct CacheSpan {
   int32_t tok0, n, S;  // first query row, queries, tokens (clamped to what the buffers hold)
@@ -85,12 +95,17 @@ __device__ __forceinline__ CacheSpan cache_span(const CacheAttnParams& p, int r)
   return s;
 }
 
+__device__ __forceinline__ UDiv cold_div(const __attribute__((address_space(4))) UDiv& d) { return {d.m, d.l}; }
+__device__ __forceinline__ CacheMask cold_mask(ColdArgs a) {
+  return {a->mask.causal, a->mask.window, a->mask.dil, a->mask.blk, a->mask.prefix, cold_div(a->mask.div_blk), cold_div(a->mask.div_dil)};
+}
+
 // Positions of the queries of row tile rt (ROWS rows) and its walk.
 template <int ROWS>
-__device__ __forceinline__ TileWalk cache_walk_of(const CacheAttnParams& p, const CacheSpan& s, int rt) {
-  const int t0 = udiv(rt * ROWS, p.div_g), t1 = imin32(udiv(rt * ROWS + ROWS - 1, p.div_g), s.n - 1);
+__device__ __forceinline__ TileWalk cache_walk_of(const CacheMask& m, UDiv div_g, const CacheSpan& s, int rt) {
+  const int t0 = udiv(rt * ROWS, div_g), t1 = imin32(udiv(rt * ROWS + ROWS - 1, div_g), s.n - 1);
   const int32_t at = s.S - s.n;
-  return cache_tile_walk(p.mask, at + t0, at + t1, s.S, ROWS == 128 ? 64 : 32);
+  return cache_tile_walk(m, at + t0, at + t1, s.S, ROWS == 128 ? 64 : 32);
 }
 
 template <int FMT, bool HI>
@@ -174,8 +189,11 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
   const int n_rows = sp.n * p.G;
 
   for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
-    const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
-    const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
+    const ColdArgs ta = cold_args();
+    const CacheMask mask = cold_mask(ta);
+    const UDiv div_g = cold_div(ta->div_g);
+    const TileWalk tw = cache_walk_of<ROWS>(mask, div_g, sp, rt);
+    const int chunk = walk_chunk(tw.n, ta->parts, ta->chunk);
     const int used = (tw.n + chunk - 1) / chunk;  // parts that have steps
     if (z > 0 && z >= used) continue;             // part 0 writes the rows that see nothing
     int s0 = z * chunk, s1 = imin32(s0 + chunk, tw.n);
@@ -194,13 +212,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     for (int b = 0; b < NT; ++b) {
       const int row = row0 + 16 * b + n16;
       rok[b] = row < n_rows;
-      const int t = rok[b] ? udiv(row, p.div_g) : 0, h = hk * p.G + (rok[b] ? row - t * p.G : 0);
+      const int t = rok[b] ? udiv(row, div_g) : 0, h = hk * ta->G + (rok[b] ? row - t * ta->G : 0);
       ipos[b] = sp.S - sp.n + t;
-      rk[b] = rok[b] ? cache_row_keys(p.mask, ipos[b], sp.S) : RowKeys{0, 0, 0};
-      c1[b] = p.scale * (p.head_scale ? p.head_scale[h] : 1.f);
-      sl[b] = p.alibi ? p.alibi[h] : 0.f;
+      rk[b] = rok[b] ? cache_row_keys(mask, ipos[b], sp.S) : RowKeys{0, 0, 0};
+      c1[b] = ta->scale * (ta->head_scale ? ta->head_scale[h] : 1.f);
+      sl[b] = ta->alibi ? ta->alibi[h] : 0.f;
       if constexpr (SCORE == CACHE_SOFTMAX) c1[b] *= kCLog2e;
-      const uint16_t* qp = p.q + (int64_t)(sp.tok0 + t) * p.q_st + (int64_t)h * p.q_sh;
+      const uint16_t* qp = ta->q + (int64_t)(sp.tok0 + t) * ta->q_st + (int64_t)h * ta->q_sh;
       otok[b] = sp.tok0 + t;
       ohead[b] = h;
 #pragma unroll
@@ -222,23 +240,24 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
 
     // Page numbers and scales of 64 pages from pg0 on, one per lane; a step's two
     // halves are always among them.
-    auto pages_from = [&](int pg) {
+    auto pages_from = [&](int pg) __attribute__((always_inline)) {
+      const ColdArgs a = cold_args();
       pg0 = pg;
       const int at = pg + lane;
-      pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
+      pg_id = at < a->width ? cache_page(a->table[(int64_t)r * a->table_stride + at], a->num_blocks) : -1;
       const int64_t id = imax32(pg_id, 0);
-      pg_ks = p.ks[id * p.ks_sb + hk * p.ks_sh];
-      pg_vs = p.vs[id * p.vs_sb + hk * p.vs_sh];
+      pg_ks = a->ks[id * a->ks_sb + hk * a->ks_sh];
+      pg_vs = a->vs[id * a->vs_sb + hk * a->vs_sh];
     };
     const uint32_t k_off = (uint32_t)(n16 * (int32_t)p.k_st + 16 * g);
     const uint32_t v_off = (uint32_t)(4 * g * (int32_t)p.v_st + n16 * DC);
-    auto pages_of = [&](int key) {
+    auto pages_of = [&](int key) __attribute__((always_inline)) {
       const int pg = key >> p.bshift, last = (key + 16) >> p.bshift;
       if (pg < pg0 || last - pg0 > 63) pages_from(pg);
     };
     CacheKeys<D> kk;
     CacheValues<D> vv;
-    auto issue_k = [&](int s) {
+    auto issue_k = [&](int s) __attribute__((always_inline)) {
       kk.key = walk_key(tw, s);
       pages_of(kk.key);
 #pragma unroll
@@ -252,7 +271,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
         for (int c = 0; c < W64; ++c) kk.w[t][c] = *(const cu32x4_t*)(kp + k_off + 64 * c);
       }
     };
-    auto issue_v = [&](int s) {  // after issue_k of the same step
+    auto issue_v = [&](int s) __attribute__((always_inline)) {  // after issue_k of the same step
       const int key = walk_key(tw, s);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -278,7 +297,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     // rows that see them is added first: NaN where a row sees a NaN (a product of
     // 1 at those codes with 1 at the keys that it sees), and an infinity of e5m2,
     // as 2^120, by the row's weights, grown until it is one.
-    auto clean = [&](const uint32_t (&vis)[NT], const uint32_t (&pw)[NT][4], const float (&vs)[2], float (&v2)[2]) {
+    auto clean = [&](const uint32_t (&vis)[NT], const uint32_t (&pw)[NT][4], const float (&vs)[2], float (&v2)[2]) __attribute__((always_inline)) {
       uint32_t bad = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -341,7 +360,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
 
     // One step: its scores from K (whose registers then take the next step's),
     // weights, and the second product from V.
-    auto compute = [&](int s) {
+    auto compute = [&](int s) __attribute__((always_inline)) {
       f32x4_t sc[NT][2];  // lane: row n16 of each block, keys key + 16 t + 4 g + e
       const int key = kk.key;
       float ks[2], vs[2];  // before the next step's pages take their place
@@ -366,8 +385,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       }
       if (s + 1 < s1) issue_k(s + 1);
       const bool full = walk_full(tw, key, 32) && pok[0] && pok[1];
-      const int dres = p.mask.dil > 1 ? key - udiv(key, p.mask.div_dil) * p.mask.dil : 0;  // key % dil
-      // vs = 2^e mant: the power goes to V's conversion, mant (1 for a power of two) to P
+            // vs = 2^e mant: the power goes to V's conversion, mant (1 for a power of two) to P
       float v2[2], mant[2], inv[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -388,16 +406,20 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
         vis[b] = 0xffu;
         if (!full) {
           vis[b] = 0;
-          const int ires = p.mask.dil > 1 && ipos[b] >= 0 ? ipos[b] - udiv(ipos[b], p.mask.div_dil) * p.mask.dil : 0;
+          const ColdArgs a = cold_args();
+          const int dil = a->mask.dil;
+          const UDiv div = {a->mask.div_dil.m, a->mask.div_dil.l};
+          const int dres = dil > 1 ? key - udiv(key, div) * dil : 0;  // key % dil
+          const int ires = dil > 1 && ipos[b] >= 0 ? ipos[b] - udiv(ipos[b], div) * dil : 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int d = 16 * t + 4 * g + e, j = key + d;
               bool ok = j >= rk[b].lo && j < rk[b].hi;
-              if (p.mask.dil > 1) {
+              if (dil > 1) {
                 const int jr = dres + d;  // (key % dil) + d, reduced
-                ok = ok && jr - udiv(jr, p.mask.div_dil) * p.mask.dil == ires;
+                ok = ok && jr - udiv(jr, div) * dil == ires;
               }
               ok = (ok || j < rk[b].pre) && pok[t];
               vis[b] |= (ok ? 1u : 0u) << (4 * t + e);
@@ -512,6 +534,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
         l_run[b] += __shfl_xor(l_run[b], 32);
       }
 
+    const ColdArgs ca = cold_args();
     const bool whole = used <= 1;  // this workgroup has all the keys of its rows
     // merge the four wavefronts' keys
     float* ml = lds + 4 * ROWS * LP;  // [4][ROWS][2]
@@ -567,20 +590,20 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       if (!rok[b]) continue;
       const int at = DC * (4 * g + wave);
       if (whole) {
-        const float f = SOFTMAX ? (l_all[b] != 0.f ? 1.f / l_all[b] : 0.f) : p.post_scale;
-        uint16_t* op = p.o + (int64_t)otok[b] * p.o_st + (int64_t)ohead[b] * p.o_sh + at;
+        const float f = SOFTMAX ? (l_all[b] != 0.f ? 1.f / l_all[b] : 0.f) : ca->post_scale;
+        uint16_t* op = ca->o + (int64_t)otok[b] * ca->o_st + (int64_t)ohead[b] * ca->o_sh + at;
         if constexpr (DC == 8)
           *(cu32x4_t*)op = cu32x4_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f),
                                     cpack(sum[1][0] * f, sum[1][1] * f), cpack(sum[1][2] * f, sum[1][3] * f)};
         else
           *(cu32x2_t*)op = cu32x2_t{cpack(sum[0][0] * f, sum[0][1] * f), cpack(sum[0][2] * f, sum[0][3] * f)};
       } else {
-        const int64_t row = ((int64_t)z * p.T + otok[b]) * p.H + ohead[b];
+        const int64_t row = ((int64_t)z * ca->T + otok[b]) * ca->H + ohead[b];
 #pragma unroll
-        for (int c = 0; c < DC / 4; ++c) *(f32x4_t*)(p.part_o + row * D + at + 4 * c) = sum[c];
+        for (int c = 0; c < DC / 4; ++c) *(f32x4_t*)(ca->part_o + row * D + at + 4 * c) = sum[c];
         if (SOFTMAX && g == 0 && wave == 0) {
-          p.part_ml[2 * row] = m_all[b];
-          p.part_ml[2 * row + 1] = l_all[b];
+          ca->part_ml[2 * row] = m_all[b];
+          ca->part_ml[2 * row + 1] = l_all[b];
         }
       }
     }

@@ -63,7 +63,6 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
   const CacheSpan sp = cache_span(p, r);
   const int n_rows = sp.n * p.G;
   const int bs_mask = (1 << p.bshift) - 1;
-  const int32_t* table = p.table + (int64_t)r * p.table_stride;
   const uint8_t* kbase = p.k + hk * p.k_sh;
   const uint8_t* vbase = p.v + hk * p.v_sh;
 
@@ -85,23 +84,26 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
   constexpr int SW8 = D == 128 ? 32 : 16;  // 16 row_swz(8): rows 8 further on flip this bit of the slot
 
   for (int rt = rt0; rt * ROWS < n_rows; rt += p.tiles) {
-    const TileWalk tw = cache_walk_of<ROWS>(p, sp, rt);
-    const int chunk = walk_chunk(tw.n, p.parts, p.chunk);
+    const ColdArgs ta = cold_args();
+    const CacheMask mask = cold_mask(ta);
+    const UDiv div_g = cold_div(ta->div_g);
+    const TileWalk tw = cache_walk_of<ROWS>(mask, div_g, sp, rt);
+    const int chunk = walk_chunk(tw.n, ta->parts, ta->chunk);
     const int used = (tw.n + chunk - 1) / chunk;
     if (z > 0 && z >= used) continue;  // part 0 writes the rows that see nothing
     const int s0 = z * chunk, s1 = imin32(s0 + chunk, tw.n);
 
     const int row = rt * ROWS + 32 * wave + lq;
     const bool rok = row < n_rows;
-    const int t = rok ? udiv(row, p.div_g) : 0, h = hk * p.G + (rok ? row - t * p.G : 0);
+    const int t = rok ? udiv(row, div_g) : 0, h = hk * ta->G + (rok ? row - t * ta->G : 0);
     const int ipos = sp.S - sp.n + t;
-    const RowKeys rk = rok ? cache_row_keys(p.mask, ipos, sp.S) : RowKeys{0, 0, 0};
-    float c1 = p.scale * (p.head_scale ? p.head_scale[h] : 1.f);
-    const float sl = p.alibi ? p.alibi[h] : 0.f;
+    const RowKeys rk = rok ? cache_row_keys(mask, ipos, sp.S) : RowKeys{0, 0, 0};
+    float c1 = ta->scale * (ta->head_scale ? ta->head_scale[h] : 1.f);
+    const float sl = ta->alibi ? ta->alibi[h] : 0.f;
     if constexpr (SCORE == CACHE_SOFTMAX) c1 *= kCLog2e;
     bf16x8_t qf[DK];
     {
-      const uint16_t* qp = p.q + (int64_t)(sp.tok0 + t) * p.q_st + (int64_t)h * p.q_sh + 8 * here(lh);
+      const uint16_t* qp = ta->q + (int64_t)(sp.tok0 + t) * ta->q_st + (int64_t)h * ta->q_sh + 8 * here(lh);
 #pragma unroll
       for (int kk = 0; kk < DK; ++kk) {
         const u32x4_t w = *(const u32x4_t*)(qp + 16 * kk);
@@ -112,15 +114,16 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
     // pages: numbers and scales of 64 from pg0 on, one per lane (every wavefront its own)
     int32_t pg0 = 1 << 30, pg_id = -1;
     float pg_ks = 0.f, pg_vs = 0.f;
-    auto pages_of = [&](int key) {
+    auto pages_of = [&](int key) __attribute__((always_inline)) {
       const int pg = key >> p.bshift, last = (key + BN - 16) >> p.bshift;
       if (pg >= pg0 && last - pg0 <= 63) return;
+      const ColdArgs a = cold_args();
       pg0 = pg;
       const int at = pg + here(lane);
-      pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
+      pg_id = at < a->width ? cache_page(a->table[(int64_t)r * a->table_stride + at], a->num_blocks) : -1;
       const int64_t id = imax32(pg_id, 0);
-      pg_ks = p.ks[id * p.ks_sb + hk * p.ks_sh];
-      pg_vs = p.vs[id * p.vs_sb + hk * p.vs_sh];
+      pg_ks = a->ks[id * a->ks_sb + hk * a->ks_sh];
+      pg_vs = a->vs[id * a->vs_sb + hk * a->vs_sh];
     };
     // what belongs to the four 16-key groups of a tile: of the one in the
     // registers (next) and of the one in LDS that is computed (cur)
@@ -133,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
     };
     Groups next, cur;
     cu32x4_t kr[NL], vr[NL];
-    auto load = [&](int s) {
+    auto load = [&](int s) __attribute__((always_inline)) {
       next.key = walk_key(tw, s);
       pages_of(next.key);
 #pragma unroll
@@ -146,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
         vr[n] = *(const cu32x4_t*)(vbase + page * p.v_sb + place * p.v_st + v_off);
       }
     };
-    auto scales = [&]() {  // of the tile that load() has asked for
+    auto scales = [&]() __attribute__((always_inline)) {  // of the tile that load() has asked for
       next.full = walk_full(tw, next.key, BN);
       if (p.bshift >= 6) {  // one page
         const int at = (next.key >> p.bshift) - pg0;
@@ -210,17 +213,20 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
       if (!RAW && !next.full && bad) poison_s = 1;
     };
     // bit e: the row sees key jb + 4 lh + 8 (e / 4) + e % 4
-    auto seen = [&](int jb, bool ok0, bool ok1) {
+    auto seen = [&](int jb, bool ok0, bool ok1) __attribute__((always_inline)) {
+      const ColdArgs a = cold_args();
+      const int dil = a->mask.dil;
+      const UDiv div = {a->mask.div_dil.m, a->mask.div_dil.l};
       uint32_t vis = 0;
-      const int dres = p.mask.dil > 1 ? jb - udiv(jb, p.mask.div_dil) * p.mask.dil : 0;
-      const int ires = p.mask.dil > 1 && ipos >= 0 ? ipos - udiv(ipos, p.mask.div_dil) * p.mask.dil : 0;
+      const int dres = dil > 1 ? jb - udiv(jb, div) * dil : 0;
+      const int ires = dil > 1 && ipos >= 0 ? ipos - udiv(ipos, div) * dil : 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int d = 4 * lh + 8 * (e >> 2) + (e & 3), j = jb + d;
         bool ok = j >= rk.lo && j < rk.hi;
-        if (p.mask.dil > 1) {
+        if (dil > 1) {
           const int jr = dres + d;
-          ok = ok && jr - udiv(jr, p.mask.div_dil) * p.mask.dil == ires;
+          ok = ok && jr - udiv(jr, div) * dil == ires;
         }
         ok = (ok || j < rk.pre) && (e < 8 ? ok0 : ok1);
         vis |= (ok ? 1u : 0u) << e;
@@ -247,8 +253,9 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
       for (int e = 0; e < 16; ++e) s[e] = 0.f;
       __builtin_amdgcn_s_setprio(1);
       bf16x8_t kf[DK];
+      const int kl = here(k_lane);
 #pragma unroll
-      for (int kk = 0; kk < DK; ++kk) kf[kk] = *(const bf16x8_t*)(Kb + (k_lane ^ (32 * kk)));
+      for (int kk = 0; kk < DK; ++kk) kf[kk] = *(const bf16x8_t*)(Kb + (kl ^ (32 * kk)));
 #pragma unroll
       for (int kk = 0; kk < DK; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf[kk], s, 0, 0, 0);
       // four LDS reads ahead of the MFMAs
@@ -261,13 +268,14 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
       __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
       __builtin_amdgcn_s_setprio(0);
       // V^T of the block's first 16 keys, on its way while the weights are made
+      const int vl = here(v_lane);
       bf16x8_t vf[2][DB];
       auto read_v = [&](int half) __attribute__((always_inline)) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const char* pa = Kb + 16 * half * RP;
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (v_lane ^ (64 * db))));
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (v_lane ^ (64 * db) ^ SW8)));
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (vl ^ (64 * db))));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (vl ^ (64 * db) ^ SW8)));
           vf[half][db] = __builtin_bit_cast(bf16x8_t, (i16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
       };
@@ -434,9 +442,10 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
 
     if constexpr (SOFTMAX) l_run = xhalf_sum(l_run);
     if (rok) {
+      const ColdArgs a = cold_args();
       if (used <= 1) {
-        const float f = SOFTMAX ? (l_run != 0.f ? 1.f / l_run : 0.f) : p.post_scale;
-        uint16_t* op = p.o + (int64_t)(sp.tok0 + t) * p.o_st + (int64_t)h * p.o_sh + 4 * here(lh);
+        const float f = SOFTMAX ? (l_run != 0.f ? 1.f / l_run : 0.f) : a->post_scale;
+        uint16_t* op = a->o + (int64_t)(sp.tok0 + t) * a->o_st + (int64_t)h * a->o_sh + 4 * here(lh);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -444,16 +453,16 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
             *(u32x2_t*)(op + 32 * db + 8 * q) = u32x2_t{pack_bf16x2(acc[db][4 * q] * f, acc[db][4 * q + 1] * f),
                                                        pack_bf16x2(acc[db][4 * q + 2] * f, acc[db][4 * q + 3] * f)};
       } else {
-        const int64_t at = ((int64_t)z * p.T + sp.tok0 + t) * p.H + h;
-        float* op = p.part_o + at * D + 4 * here(lh);
+        const int64_t at = ((int64_t)z * a->T + sp.tok0 + t) * a->H + h;
+        float* op = a->part_o + at * D + 4 * here(lh);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             *(f32x4_t*)(op + 32 * db + 8 * q) = f32x4_t{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2], acc[db][4 * q + 3]};
         if (SOFTMAX && lh == 0) {
-          p.part_ml[2 * at] = m_run;
-          p.part_ml[2 * at + 1] = l_run;
+          a->part_ml[2 * at] = m_run;
+          a->part_ml[2 * at + 1] = l_run;
         }
       }
     }
