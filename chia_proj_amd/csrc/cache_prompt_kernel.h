@@ -241,53 +241,21 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
       for (int e = 0; e < 16; ++e) acc[db][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    // one 32-key block of the tile in LDS at `st`
-    auto block = [&](const char* st, int kb) __attribute__((always_inline)) {
-      const float ks2[2] = {sel(kb, cur.ks[0], cur.ks[2]), sel(kb, cur.ks[1], cur.ks[3])};
-      const float vs2[2] = {sel(kb, cur.vs[0], cur.vs[2]), sel(kb, cur.vs[1], cur.vs[3])};
-      const bool ok2[2] = {sel(kb, cur.ok[0], cur.ok[2]), sel(kb, cur.ok[1], cur.ok[3])};
-      const int jb = cur.key + 32 * kb;
-      const char* Kb = st + 32 * kb * RP;
+    // The 16 scores of a 32-key block as the matrix cores give them.
+    auto products = [&](const char* Kb) __attribute__((always_inline)) {
       f32x16_t s;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0.f;
-      __builtin_amdgcn_s_setprio(1);
       bf16x8_t kf[DK];
       const int kl = here(k_lane);
 #pragma unroll
       for (int kk = 0; kk < DK; ++kk) kf[kk] = *(const bf16x8_t*)(Kb + (kl ^ (32 * kk)));
 #pragma unroll
       for (int kk = 0; kk < DK; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf[kk], s, 0, 0, 0);
-      // four LDS reads ahead of the MFMAs
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-      for (int kk = 4; kk < DK; ++kk) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-      __builtin_amdgcn_s_setprio(0);
-      // V^T of the block's first 16 keys, on its way while the weights are made
-      const int vl = here(v_lane);
-      bf16x8_t vf[2][DB];
-      auto read_v = [&](int half) __attribute__((always_inline)) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const char* pa = Kb + 16 * half * RP;
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (vl ^ (64 * db))));
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (vl ^ (64 * db) ^ SW8)));
-          vf[half][db] = __builtin_bit_cast(bf16x8_t, (i16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-      };
-      read_v(0);
-      __builtin_amdgcn_sched_barrier(0);
-      // key of register e: jb + 4 lh + 8 (e / 4) + e % 4; e < 8: the block's first group of 16
-      if (cur.frac)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] *= fraction_of(ks2[e >> 3]);
-      uint32_t vis = 0xffffu;
-      if (!cur.full) vis = seen(jb, ok2[0], ok2[1]);
-      asm("" : "+v"(vis));  // one register, not sixteen
+      return s;
+    };
+    // Score modifiers, in place; softmax in log2 units over kq.
+    auto modify = [&](f32x16_t& s, int jb) __attribute__((always_inline)) {
       if constexpr (SCORE != CACHE_SOFTMAX) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -299,7 +267,105 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
           s[e] = SCORE == CACHE_SOFTMAX_MOD ? v * kCLog2e : v;
         }
       }
-      const float kq = SCORE == CACHE_SOFTMAX ? c1 : 1.f;  // s kq: the score in log2 units (softmax)
+    };
+    const float kq = SCORE == CACHE_SOFTMAX ? c1 : 1.f;  // s kq: the score in log2 units (softmax)
+    auto weight = [&](float v) __attribute__((always_inline)) {  // sigmoid, ReLU
+      if constexpr (SCORE == CACHE_SIGMOID)
+        return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kCLog2e * (v + p.bias)));
+      else
+        return v < 0.f ? 0.f : v;
+    };
+    // raises the running maximum if `mx`, of this lane's scores, exceeds it by more than 8
+    auto raise = [&](float mx) __attribute__((always_inline)) {
+      mx = xhalf_max(mx) * kq;
+      const float m_new = mx > m_run + kCLazy ? mx : m_run;
+      if (__any(m_new != m_run)) {
+        const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= a;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[db][e] *= a;
+        m_run = m_new;
+      }
+    };
+    // V^T of 16 keys
+    auto read_v = [&](const char* Vb, int vl, bf16x8_t (&vf)[DB]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(Vb + (vl ^ (64 * db))));
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(Vb + 8 * RP + (vl ^ (64 * db) ^ SW8)));
+        vf[db] = __builtin_bit_cast(bf16x8_t, (i16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    };
+    auto add_pv = [&](const bf16x8_t (&vf)[DB], const uint32_t* pk) __attribute__((always_inline)) {
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, u32x4_t{pk[0], pk[1], pk[2], pk[3]});
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db], pf, acc[db], 0, 0, 0);
+    };
+
+    // A tile that every row sees whole, of scales that are powers of two: both blocks
+    // together, so that the second block's products run beside the first one's weights
+    // and the first one's second product beside the second's weights.
+    auto whole_tile = [&](const char* st) __attribute__((always_inline)) {
+      f32x16_t s[2];
+      s[0] = products(st);
+      s[1] = products(st + 32 * RP);
+      modify(s[0], cur.key);
+      modify(s[1], cur.key + 32);
+      float mo = 0.f;
+      if constexpr (SOFTMAX) {
+        float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fmaxf(s[0][e], s[1][e]));
+        raise(mx);
+        mo = m_run == -INFINITY ? 0.f : -m_run;
+      }
+      const int vl = here(v_lane);
+      bf16x8_t vf[2][DB];
+      read_v(st, vl, vf[0]);
+      float ls[2] = {0.f, 0.f};
+      uint32_t pk[2][8];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          float a = s[kb][2 * w], b = s[kb][2 * w + 1];
+          if constexpr (SOFTMAX) {
+            a = __builtin_amdgcn_exp2f(__builtin_fmaf(a, kq, mo));
+            b = __builtin_amdgcn_exp2f(__builtin_fmaf(b, kq, mo));
+          } else {
+            a = weight(a);
+            b = weight(b);
+          }
+          const bf16x2_t pb = pack2(a, b);
+          if constexpr (SOFTMAX) ls[kb] = __builtin_amdgcn_fdot2_f32_bf16(pb, kOnes2, ls[kb], false);
+          pk[kb][w] = __builtin_bit_cast(uint32_t, pb);
+        }
+        read_v(st + (32 * kb + 16) * RP, vl, vf[1]);
+        add_pv(vf[0], &pk[kb][0]);
+        if (kb == 0) read_v(st + 32 * RP, vl, vf[0]);
+        add_pv(vf[1], &pk[kb][4]);
+      }
+      if constexpr (SOFTMAX) l_run += ls[0] + ls[1];
+    };
+
+    // One 32-key block of any other tile.
+    auto block = [&](const char* st, int kb) __attribute__((always_inline)) {
+      const float ks2[2] = {sel(kb, cur.ks[0], cur.ks[2]), sel(kb, cur.ks[1], cur.ks[3])};
+      const float vs2[2] = {sel(kb, cur.vs[0], cur.vs[2]), sel(kb, cur.vs[1], cur.vs[3])};
+      const bool ok2[2] = {sel(kb, cur.ok[0], cur.ok[2]), sel(kb, cur.ok[1], cur.ok[3])};
+      const int jb = cur.key + 32 * kb;
+      const char* Kb = st + 32 * kb * RP;
+      f32x16_t s = products(Kb);
+      // key of register e: jb + 4 lh + 8 (e / 4) + e % 4; e < 8: the block's first group of 16
+      if (cur.frac)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= fraction_of(ks2[e >> 3]);
+      uint32_t vis = 0xffffu;
+      if (!cur.full) vis = seen(jb, ok2[0], ok2[1]);
+      asm("" : "+v"(vis));  // one register, not sixteen
+      modify(s, jb);
       uint32_t pk[8];
       if constexpr (SOFTMAX) {
         if (!cur.full)
@@ -308,30 +374,13 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
         float mx = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-        mx = xhalf_max(mx) * kq;
-        const float m_new = mx > m_run + kCLazy ? mx : m_run;
-        if (__any(m_new != m_run)) {
-          const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
-          l_run *= a;
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[db][e] *= a;
-          m_run = m_new;
-        }
+        raise(mx);
         const float mo = m_run == -INFINITY ? 0.f : -m_run;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kq, mo));
       } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float v = s[e];
-          if constexpr (SCORE == CACHE_SIGMOID)
-            v = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kCLog2e * (v + p.bias)));
-          else
-            v = v < 0.f ? 0.f : v;
-          s[e] = cur.full || ((vis >> e) & 1) ? v : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = cur.full || ((vis >> e) & 1) ? weight(s[e]) : 0.f;
       }
       float inv[2] = {1.f, 1.f};
       if (cur.frac) {
@@ -351,17 +400,13 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
         pk[w] = __builtin_bit_cast(uint32_t, pb);
       }
       if constexpr (SOFTMAX) l_run = __builtin_fmaf(ls[0], inv[0], __builtin_fmaf(ls[1], inv[1], l_run));
-
-      read_v(1);
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(1);
+      const int vl = here(v_lane);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, u32x4_t{pk[4 * half], pk[4 * half + 1], pk[4 * half + 2], pk[4 * half + 3]});
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[half][db], pf, acc[db], 0, 0, 0);
+        bf16x8_t vf[DB];
+        read_v(Kb + 16 * half * RP, vl, vf);
+        add_pv(vf, &pk[4 * half]);
       }
-      __builtin_amdgcn_s_setprio(0);
     };
 
     if (s0 < s1) {
@@ -377,8 +422,12 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
         const bool more = s + 1 < s1;
         if (more) load(s + 1);
         const int stage = (s - s0) & 1;
+        if (cur.full && !cur.frac) {
+          whole_tile(lds + stage * STAGE);
+        } else {
 #pragma unroll 1
-        for (int kb = 0; kb < 2; ++kb) block(lds + stage * STAGE, kb);
+          for (int kb = 0; kb < 2; ++kb) block(lds + stage * STAGE, kb);
+        }
         if (more) {
           scales();
           store(stage ^ 1, BoolTag<false>());
