@@ -35,20 +35,40 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnParams 
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     if (ok) {
-      if constexpr (SOFTMAX) {
-#pragma unroll 4
-        for (int z = zi; z < used; z += ZG) m = fmaxf(m, p.part_ml[2 * (z * th + at)]);
-#pragma unroll 4
-        for (int z = zi; z < used; z += ZG) {
-          const float mz = p.part_ml[2 * (z * th + at)];
-          const float w = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - m);
-          l = __builtin_fmaf(w, p.part_ml[2 * (z * th + at) + 1], l);
-          // a part that saw no key has zeros
-          sum += w * *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+      // four parts' numbers on their way at a time
+      for (int z0 = zi; z0 < used; z0 += 4 * ZG) {
+        float mz[4], lz[4];
+        f32x4_t oz[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int z = z0 + i * ZG;
+          mz[i] = -INFINITY;
+          lz[i] = 0.f;
+          oz[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          if (z < used) {
+            oz[i] = *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+            if constexpr (SOFTMAX) {
+              mz[i] = p.part_ml[2 * (z * th + at)];
+              lz[i] = p.part_ml[2 * (z * th + at) + 1];
+            }
+          }
         }
-      } else {
-#pragma unroll 4
-        for (int z = zi; z < used; z += ZG) sum += *(const f32x4_t*)(p.part_o + (z * th + at) * D + d);
+        if constexpr (SOFTMAX) {
+          const float all = fmaxf(fmaxf(fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3])), m);
+          const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - all);
+          m = all;
+          l *= f;
+          sum *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // a part that saw no key has zeros
+            const float w = mz[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz[i] - m);
+            l = __builtin_fmaf(w, lz[i], l);
+            sum += w * oz[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += oz[i];
+        }
       }
     }
     if constexpr (ZG > 1) {
@@ -120,7 +140,7 @@ int validate(const chia_cache_attn_args* a) {
 // The launch: which row tile, how many of them per (request, K/V head), and how
 // the steps of a tile's walk are split.
 struct Shape {
-  int tile;
+  int tile, waves;
   int64_t tiles, parts, chunk;
 };
 
@@ -179,6 +199,19 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   }
   if (parts > steps / least) parts = steps / least;
   if (parts < 1) parts = 1;
+  // Eight wavefronts to a workgroup where the parts are few: the same wavefronts per
+  // CU in one workgroup instead of two, with half the parts to join, or none (16-row tiles,
+  // us with four and eight: 32 requests under a window of 1024, 8 heads D128, 20.3 (2 parts), 17.9 (1); 4 of
+  // 17848, 16 heads D128, 54, 52; 11 of 32318, 8 heads D64, 69, 64; 56 of 397, 2 heads D64, 7.8, 7.1).
+  s.waves = 4;
+  if (small && steps > 8 && (groups <= 128 || (groups <= kCUs && parts <= 2))) {
+    s.waves = 8;
+    parts = (t->head_dim == 64 ? 2 : 1) * kCUs / groups;
+    if (groups > 128) parts = 1;
+    const int64_t most = steps / (groups * steps <= 2048 && steps > 32 ? 8 : 12);
+    if (parts > most) parts = most;
+    if (parts < 1) parts = 1;
+  }
   s.chunk = (steps + parts - 1) / parts;
   s.parts = (steps + s.chunk - 1) / s.chunk;
   return s;
@@ -308,11 +341,11 @@ extern "C" int chia_cache_attn(const chia_cache_attn_args* a, void* stream) {
                     : t->norm == CHIA_ATTN_NORM_RELU  ? CACHE_RELU
                     : t->alibi_slopes || t->softcap > 0.f ? CACHE_SOFTMAX_MOD : CACHE_SOFTMAX;
   const CacheAttnFn fn = s.tile == CACHE_ROWS128 ? select_cache_prompt_kernel((int)t->head_dim, (int)a->format, score)
-                         : t->head_dim == 64     ? select_cache_kernel_d64((int)a->format, score, s.tile)
-                                                 : select_cache_kernel_d128((int)a->format, score, s.tile);
+                         : t->head_dim == 64     ? select_cache_kernel_d64((int)a->format, score, s.tile, s.waves)
+                                                 : select_cache_kernel_d128((int)a->format, score, s.tile, s.waves);
   if (!fn) return CHIA_ATTN_ERR_NORM;
   void* kargs[] = {&p};
-  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)wgs), dim3(256), kargs, 0,
+  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)wgs), dim3(64 * (unsigned)s.waves), kargs, 0,
                                    (hipStream_t)stream);
   if (err == hipSuccess && s.parts > 1) {
     const Merge m = merge_kernel((int)t->head_dim, t->norm == CHIA_ATTN_NORM_SOFTMAX, s.tile, s.parts >= 8);

@@ -2,5 +2,7 @@
 #include "cache_attn_kernel.h"
 
 namespace chia {
-CacheAttnFn select_cache_kernel_d64(int format, int score, int tile) { return pick_cache_kernel<64>(format, score, tile); }
+CacheAttnFn select_cache_kernel_d64(int format, int score, int tile, int waves) {
+  return pick_cache_kernel<64>(format, score, tile, waves);
+}
 }  // namespace chia

@@ -22,8 +22,8 @@
 // sum adds the rounded weights.  The softmax maximum moves only when a score
 // exceeds it by more than 8 (log2), which one vote per step finds out.
 //
-// Rows come in tiles of 16 NT; the four wavefronts of a workgroup split a tile's
-// keys and merge through LDS.  The keys are further split over workgroups
+// Rows come in tiles of 16 NT; the NW wavefronts of a workgroup split a tile's keys
+// and merge through LDS.  The keys are further split over workgroups
 // (cache_geom.h), whose partial rows a second kernel joins.  Prompts, with many
 // rows to a K/V head, have a kernel of their own (cache_prompt_kernel.h).
 #pragma once
@@ -148,15 +148,15 @@ struct CacheValues {
   uint32_t w[8][D / 64];
 };
 
-template <int D, int FMT, int SCORE, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const CacheAttnParams p) {
+template <int D, int FMT, int SCORE, int NT, int NW>
+__global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void cache_attn_kernel(const CacheAttnParams p) {
   constexpr int KS = D / 32;            // k-steps of the first product
   constexpr int DC = D / 16;            // 16-row blocks of O^T; columns per lane of V
   constexpr int W64 = D / 64;
   constexpr int ROWS = 16 * NT;
   constexpr bool SOFTMAX = SCORE == CACHE_SOFTMAX || SCORE == CACHE_SOFTMAX_MOD;
   constexpr int LP = D + 4;             // LDS row pitch: rows start in other banks
-  __shared__ __attribute__((aligned(16))) float lds[4 * ROWS * LP + 4 * ROWS * 2];
+  __shared__ __attribute__((aligned(16))) float lds[NW * ROWS * LP + NW * ROWS * 2];
 
   const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
   float pg_ks = 0.f, pg_vs = 0.f;
   if (p.mask.window == 0 && p.mask.blk == 0) {
     int first = z * p.chunk;
-    if (((p.chunk * 32) >> p.bshift) > 63) first += wave * ((p.chunk + 3) >> 2);
+    if (((p.chunk * 32) >> p.bshift) > 63) first += wave * ((p.chunk + NW - 1) / NW);
     pg0 = (first * 32) >> p.bshift;
     const int at = pg0 + lane;
     pg_id = at < p.width ? cache_page(table[at], p.num_blocks) : -1;
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
     const int used = (tw.n + chunk - 1) / chunk;  // parts that have steps
     if (z > 0 && z >= used) continue;             // part 0 writes the rows that see nothing
     int s0 = z * chunk, s1 = imin32(s0 + chunk, tw.n);
-    const int row0 = rt * ROWS, per = (s1 - s0 + 3) >> 2;
+    const int row0 = rt * ROWS, per = (s1 - s0 + NW - 1) / NW;
     s0 = imin32(s0 + wave * per, s1);
     s1 = imin32(s0 + per, s1);
 
@@ -536,8 +536,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
 
     const ColdArgs ca = cold_args();
     const bool whole = used <= 1;  // this workgroup has all the keys of its rows
-    // merge the four wavefronts' keys
-    float* ml = lds + 4 * ROWS * LP;  // [4][ROWS][2]
+    // merge the wavefronts' keys
+    float* ml = lds + NW * ROWS * LP;  // [NW][ROWS][2]
     if constexpr (SOFTMAX) {
       if (g == 0)
 #pragma unroll
@@ -553,15 +553,15 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       m_all[b] = -INFINITY;
       l_all[b] = 0.f;
       if constexpr (SOFTMAX) {
-        float mw[4], lw[4];
+        float mw[NW], lw[NW];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
           mw[w] = ml[(w * ROWS + 16 * b + n16) * 2];
           lw[w] = ml[(w * ROWS + 16 * b + n16) * 2 + 1];
           m_all[b] = fmaxf(m_all[b], mw[w]);
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < NW; ++w)
           l_all[b] += mw[w] == -INFINITY ? 0.f : lw[w] * __builtin_amdgcn_exp2f(mw[w] - m_all[b]);
         const float f = m_run[b] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[b] - m_all[b]);
 #pragma unroll
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
               f32x4_t{acc[b][c][e], acc[b][c + 1][e], acc[b][c + 2][e], acc[b][c + 3][e]};
     }
     __syncthreads();
-    // wavefront w stores the pieces e = w of every lane's rows
+    // wavefront w < 4 stores the pieces e = w of every lane's rows
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
       f32x4_t sum[DC / 4];
@@ -584,10 +584,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void cache_attn_kernel(const 
       for (int c = 0; c < DC / 4; ++c) {
         sum[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < NW; ++w)
           sum[c] += *(const f32x4_t*)(lds + (w * ROWS + 16 * b + n16) * LP + DC * (4 * g + wave) + 4 * c);
       }
-      if (!rok[b]) continue;
+      if (!rok[b] || wave >= 4) continue;
       const int at = DC * (4 * g + wave);
       if (whole) {
         const float f = SOFTMAX ? (l_all[b] != 0.f ? 1.f / l_all[b] : 0.f) : ca->post_scale;
@@ -617,15 +617,16 @@ using CacheAttnFn = void (*)(CacheAttnParams);
 enum CacheTile : int { CACHE_ROWS16 = 0, CACHE_ROWS32 = 1, CACHE_ROWS128 = 2 };
 constexpr int kCacheRows[3] = {16, 32, 128}, kCacheStep[3] = {32, 32, 64};
 
-CacheAttnFn select_cache_kernel_d64(int format, int score, int tile);
-CacheAttnFn select_cache_kernel_d128(int format, int score, int tile);
+CacheAttnFn select_cache_kernel_d64(int format, int score, int tile, int waves);
+CacheAttnFn select_cache_kernel_d128(int format, int score, int tile, int waves);
 CacheAttnFn select_cache_prompt_kernel(int head_dim, int format, int score);
 
 template <int D>
-CacheAttnFn pick_cache_kernel(int format, int score, int tile) {
+CacheAttnFn pick_cache_kernel(int format, int score, int tile, int waves) {
 #define CHIA_CACHE(F, S)                                                                          \
   if (format == F && score == S)                                                                  \
-    return tile == CACHE_ROWS16 ? cache_attn_kernel<D, F, S, 1> : cache_attn_kernel<D, F, S, 2>;
+    return tile == CACHE_ROWS32 ? cache_attn_kernel<D, F, S, 2, 4>                                \
+           : waves == 8         ? cache_attn_kernel<D, F, S, 1, 8> : cache_attn_kernel<D, F, S, 1, 4>;
 #define CHIA_CACHE_FMT(F) \
   CHIA_CACHE(F, CACHE_SOFTMAX) CHIA_CACHE(F, CACHE_SOFTMAX_MOD) CHIA_CACHE(F, CACHE_SIGMOID) CHIA_CACHE(F, CACHE_RELU)
   CHIA_CACHE_FMT(0)
