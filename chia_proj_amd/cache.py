@@ -225,6 +225,8 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     if torch.compiler.is_compiling():
         torch.ops.chia_attn.write_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots)
         return
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (k, v)):
+        raise ValueError("write_cache is forward only: k and v must not require grad")
     try:
         key = ("cache_write",) + _meta(k, v, k_cache, v_cache, k_scale, v_scale, slots)
         args = _args_cache()

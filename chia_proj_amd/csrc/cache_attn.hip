@@ -159,6 +159,10 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   s.tile = rows <= 16 ? CACHE_ROWS16 : us32 <= us128 ? CACHE_ROWS32 : CACHE_ROWS128;
   const int R = kCacheRows[s.tile];
   s.tiles = (rows + R - 1) / R;
+  // A bound on the queries that is far too wide does not make millions of empty
+  // workgroups: those there are walk more tiles.
+  const int64_t tiles_most = ((int64_t)1 << 18) / (t->batch * hkv);
+  if (s.tiles > tiles_most) s.tiles = tiles_most > 0 ? tiles_most : 1;
   // steps of the longest request's last tile
   const int64_t S = t->seqlen < (a->width * a->block_size) ? t->seqlen : a->width * a->block_size;
   const int64_t span = (R + G - 1) / G;
