@@ -392,7 +392,7 @@ def bwd_noalloc(args: BwdArgs, stream: int) -> None:
 
 
 def cache_tables(args: CacheTablesArgs, stream: int) -> None:
-    st = _load().chia_cache_tables(args, stream)
+    st = (_lib or _load()).chia_cache_tables(args, stream)
     if st != 0:
         raise ChiaAttnError(st, "chia_cache_tables")
 
@@ -404,7 +404,7 @@ def cache_release(args: CacheReleaseArgs, stream: int) -> None:
 
 
 def cache_write(args: CacheWriteArgs, stream: int) -> None:
-    st = _load().chia_cache_write(args, stream)
+    st = (_lib or _load()).chia_cache_write(args, stream)
     if st != 0:
         raise ChiaAttnError(st, "chia_cache_write")
 
@@ -417,7 +417,7 @@ def cache_attn_workspace_size(args: CacheAttnArgs) -> int:
 
 
 def cache_attn(args: CacheAttnArgs, stream: int) -> None:
-    st = _load().chia_cache_attn(args, stream)
+    st = (_lib or _load()).chia_cache_attn(args, stream)
     if st != 0:
         raise ChiaAttnError(st, "chia_cache_attn")
 

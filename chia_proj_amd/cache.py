@@ -25,8 +25,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .attention import (FP8_FORMATS, PerHead, _args_cache, _ARGS_CACHE_MAX, _check_params, _current_stream, _device_of,
-                        _head_key, _layout_ok_packed, _per_head_vector, make_args)
+from .attention import (FP8_FORMATS, PerHead, _args_cache, _ARGS_CACHE_MAX, _check_params, _current_stream, _head_key,
+                        _layout_ok_packed, _per_head_vector, make_args)
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 
@@ -131,8 +131,7 @@ def extend_block_tables(block_tables: torch.Tensor, context_lens: torch.Tensor, 
     a.slots, a.positions, a.cu_seqlens = at, at + 4 * T, at + 8 * T
     at += 8 * T + 4 * (R + 1)
     a.seq_lens, a.free_left, a.missing = at, at + 4 * R, at + 4 * R + 4
-    with _device_of(block_tables):
-        _lib.cache_tables(a, _current_stream(block_tables))
+    _launch(_lib.cache_tables, a, block_tables)
     return step
 
 
@@ -160,8 +159,7 @@ def release_block_tables(block_tables: torch.Tensor, context_lens: torch.Tensor,
                               context_lens=context_lens.data_ptr(), finished=finished.data_ptr(),
                               free_blocks=free_blocks.data_ptr(), free_count=free_count.data_ptr(),
                               free_capacity=free_blocks.shape[0], free_left=left.data_ptr())
-    with _device_of(block_tables):
-        _lib.cache_release(a, _current_stream(block_tables))
+    _launch(_lib.cache_release, a, block_tables)
     return left
 
 
@@ -201,6 +199,18 @@ def _laid_out(t: torch.Tensor) -> torch.Tensor:
     return t if _layout_ok_packed(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(call, args, t: torch.Tensor) -> None:
+    """call(args, stream) on t's device and its current stream."""
+    if _get_device() == t.get_device():
+        call(args, _current_stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            call(args, _current_stream(t))
+
+
 def _remember(cache, key, entry) -> None:
     cache[key] = entry
     if len(cache) > _ARGS_CACHE_MAX:
@@ -238,8 +248,7 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
         if not (ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3]) & 15:
             a.k, a.v, a.k_cache, a.v_cache = ptrs
             a.k_scale, a.v_scale, a.slots = k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr()
-            with _device_of(k_cache):
-                _lib.cache_write(a, _current_stream(k_cache))
+            _launch(_lib.cache_write, a, k_cache)
             return
     pages, heads, bs, D = _check_cache(k_cache, v_cache, k_scale, v_scale)
     _contiguous("slots", _vector("slots", slots, k_cache.device, (None,)))
@@ -261,8 +270,7 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     a.k_stride[:], a.v_stride[:] = k_.stride()[:2], v_.stride()[:2]
     a.k_cache_stride[:], a.v_cache_stride[:] = k_cache.stride()[:3], v_cache.stride()[:3]
     a.k_scale_stride[:], a.v_scale_stride[:] = k_scale.stride(), v_scale.stride()
-    with _device_of(k_cache):
-        _lib.cache_write(a, _current_stream(k_cache))
+    _launch(_lib.cache_write, a, k_cache)
     if key is not None and k_ is k and v_ is v:
         _remember(args, key, a)
 
@@ -330,11 +338,10 @@ def attention_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                 a.cu_seqlens = cu_seqlens.data_ptr()
             c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
             c.block_tables, c.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
-            with _device_of(q):
-                if nbytes:
-                    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-                    c.workspace = ws.data_ptr()
-                _lib.cache_attn(c, _current_stream(q))
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+                c.workspace = ws.data_ptr()
+            _launch(_lib.cache_attn, c, q)
             return o
 
     pages, hkv, bs, D = _check_cache(k_cache, v_cache, k_scale, v_scale)
@@ -384,11 +391,10 @@ def attention_cache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                            table_stride=_row_stride(block_tables), width=width, seq_lens=seq_lens.data_ptr(),
                            num_blocks=pages, queries=T, max_query=min(most_q, T), block_size=bs)
     c.k_scale_stride[:], c.v_scale_stride[:] = k_scale.stride(), v_scale.stride()
-    with _device_of(q):
-        c.workspace_bytes = nbytes = _lib.cache_attn_workspace_size(c)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        c.workspace = ws.data_ptr() if nbytes else None
-        _lib.cache_attn(c, _current_stream(q))
+    c.workspace_bytes = nbytes = _lib.cache_attn_workspace_size(c)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    c.workspace = ws.data_ptr() if nbytes else None
+    _launch(_lib.cache_attn, c, q)
     if key is not None and q_ is q:
         _remember(cache, key, (c, a, nbytes, hs, sl))
     return o
