@@ -231,6 +231,7 @@ CacheMask mask_of(const chia_attn_args* t) {
   m.prefix = t->prefix < kMaxSeq ? t->prefix : (int32_t)kMaxSeq;
   m.div_blk = make_udiv(m.blk > 0 ? m.blk : 1);
   m.div_dil = make_udiv(m.dil);
+  m.comb = cache_comb(m.dil);
   return m;
 }
 

@@ -97,7 +97,8 @@ __device__ __forceinline__ CacheSpan cache_span(const CacheAttnParams& p, int r)
 
 __device__ __forceinline__ UDiv cold_div(const __attribute__((address_space(4))) UDiv& d) { return {d.m, d.l}; }
 __device__ __forceinline__ CacheMask cold_mask(ColdArgs a) {
-  return {a->mask.causal, a->mask.window, a->mask.dil, a->mask.blk, a->mask.prefix, cold_div(a->mask.div_blk), cold_div(a->mask.div_dil)};
+  return {a->mask.causal, a->mask.window, a->mask.dil, a->mask.blk, a->mask.prefix, cold_div(a->mask.div_blk), cold_div(a->mask.div_dil),
+          a->mask.comb};
 }
 
 // Positions of the queries of row tile rt (ROWS rows) and its walk.
@@ -405,25 +406,9 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void cache_attn_kernel(co
       for (int b = 0; b < NT; ++b) {
         vis[b] = 0xffu;
         if (!full) {
-          vis[b] = 0;
-          const ColdArgs a = cold_args();
-          const int dil = a->mask.dil;
-          const UDiv div = {a->mask.div_dil.m, a->mask.div_dil.l};
-          const int dres = dil > 1 ? key - udiv(key, div) * dil : 0;  // key % dil
-          const int ires = dil > 1 && ipos[b] >= 0 ? ipos[b] - udiv(ipos[b], div) * dil : 0;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int d = 16 * t + 4 * g + e, j = key + d;
-              bool ok = j >= rk[b].lo && j < rk[b].hi;
-              if (dil > 1) {
-                const int jr = dres + d;  // (key % dil) + d, reduced
-                ok = ok && jr - udiv(jr, div) * dil == ires;
-              }
-              ok = (ok || j < rk[b].pre) && pok[t];
-              vis[b] |= (ok ? 1u : 0u) << (4 * t + e);
-            }
+          const uint32_t bits = cache_seen(cold_mask(cold_args()), rk[b], ipos[b], key) &
+                                ((pok[0] ? 0xffffu : 0u) | (pok[1] ? 0xffff0000u : 0u));
+          vis[b] = ((bits >> (4 * g)) & 0xfu) | ((bits >> (4 * g + 12)) & 0xf0u);
         }
         float x[2][4];
 #pragma unroll

@@ -24,7 +24,14 @@ CHIA_HD int32_t cache_slot(int32_t slot, int32_t num_slots) { return (uint32_t)s
 struct CacheMask {
   int32_t causal, window, dil, blk, prefix;  // window, blk, prefix below 2^28; 0 = off
   UDiv div_blk, div_dil;
+  uint32_t comb;  // bits 0, dil, 2 dil, ... below 32
 };
+
+CHIA_HD uint32_t cache_comb(int32_t dil) {
+  uint32_t bits = 1;
+  for (int32_t d = dil; d < 32; d += dil) bits |= 1u << d;
+  return bits;
+}
 
 struct RowKeys {
   int32_t lo, hi, pre;  // lo <= j < hi (and the dilation), or j < pre
@@ -44,6 +51,23 @@ CHIA_HD RowKeys cache_row_keys(const CacheMask& m, int32_t i, int32_t S) {
     hi = imin32(hi, b + m.blk);
   }
   return {lo, hi, imin32(m.prefix, S)};
+}
+
+// Bits below n, of 32.
+CHIA_HD uint32_t bits_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+// Bit d: the row at position i sees key j0 + d (j0 >= 0).  The band and the prefix are
+// ranges of bits, the dilation one comb of them, moved to the first key of i's class:
+// one division for 32 keys.
+CHIA_HD uint32_t cache_seen(const CacheMask& m, const RowKeys& k, int32_t i, int32_t j0) {
+  uint32_t bits = bits_below(k.hi - j0) & ~bits_below(k.lo - j0);
+  if (m.dil > 1) {
+    const int32_t at = imax32(i, 0);  // (a row at i < 0 sees nothing)
+    int32_t first = (at - udiv(at, m.div_dil) * m.dil) - (j0 - udiv(j0, m.div_dil) * m.dil);
+    if (first < 0) first += m.dil;
+    bits &= first < 32 ? m.comb << first : 0u;
+  }
+  return bits | bits_below(k.pre - j0);
 }
 
 // The walk of a row tile: step s covers the `step` keys from walk_key(s) on.

@@ -214,24 +214,9 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
     };
     // bit e: the row sees key jb + 4 lh + 8 (e / 4) + e % 4
     auto seen = [&](int jb, bool ok0, bool ok1) __attribute__((always_inline)) {
-      const ColdArgs a = cold_args();
-      const int dil = a->mask.dil;
-      const UDiv div = {a->mask.div_dil.m, a->mask.div_dil.l};
-      uint32_t vis = 0;
-      const int dres = dil > 1 ? jb - udiv(jb, div) * dil : 0;
-      const int ires = dil > 1 && ipos >= 0 ? ipos - udiv(ipos, div) * dil : 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = 4 * lh + 8 * (e >> 2) + (e & 3), j = jb + d;
-        bool ok = j >= rk.lo && j < rk.hi;
-        if (dil > 1) {
-          const int jr = dres + d;
-          ok = ok && jr - udiv(jr, div) * dil == ires;
-        }
-        ok = (ok || j < rk.pre) && (e < 8 ? ok0 : ok1);
-        vis |= (ok ? 1u : 0u) << e;
-      }
-      return vis;
+      const uint32_t bits = (cache_seen(cold_mask(cold_args()), rk, here(ipos), jb) &
+                             ((ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u))) >> (4 * here(lh));
+      return (bits & 0xfu) | ((bits >> 4) & 0xf0u) | ((bits >> 8) & 0xf00u) | ((bits >> 12) & 0xf000u);
     };
 
     f32x16_t acc[DB];
@@ -453,11 +438,12 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
             for (int i = 0; i < 4; ++i)
               sees[i] = ((vis >> (2 * i)) & 1 ? 0x3f80u : 0u) | ((vis >> (2 * i + 1)) & 1 ? 0x3f800000u : 0u);
             const bf16x8_t sf = __builtin_bit_cast(bf16x8_t, sees);
+            const int vl = here(v_lane);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
               const char* pa = lds + 16 * hb * RP;
-              const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (v_lane ^ (64 * db))));
-              const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (v_lane ^ (64 * db) ^ SW8)));
+              const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + (vl ^ (64 * db))));
+              const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(pa + 8 * RP + (vl ^ (64 * db) ^ SW8)));
               const i16x8_t a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
               i16x8_t nan, up, down;
 #pragma unroll

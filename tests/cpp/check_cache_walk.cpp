@@ -1,7 +1,7 @@
 // Host check of the cache attention's walk (cache_geom.h) against the mask's
 // definition: every key that some row of a tile sees is in exactly one step,
 // tiles called full are seen by every row, the parts of a split cover the steps
-// once, and page and slot numbers outside the cache are refused.
+// once, the 32-bit words of the keys that a row sees are those keys, and page and slot numbers outside the cache are refused.
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
@@ -37,6 +37,7 @@ int main() {
     m.prefix = m.dil > 1 || rnd(2) ? 0 : 1 + rnd(200);
     m.div_blk = make_udiv(m.blk > 0 ? m.blk : 1);
     m.div_dil = make_udiv(m.dil);
+    m.comb = cache_comb(m.dil);
     const int S = rnd(10) ? rnd(400) : rnd(3);
     const int n = 1 + rnd(40), i0 = S - n + rnd(n), i1 = i0 + rnd(S - i0 > 0 ? S - i0 : 1);
     if (i1 >= S && S > 0) continue;
@@ -66,6 +67,14 @@ int main() {
       if (times[j] > 1 || (any && times[j] != 1)) ++failures;
       ++checked;
     }
+    for (int i = i0; i <= i1; ++i) {
+      const RowKeys k = cache_row_keys(m, i, S);
+      for (int c = 0; c < S + 64; c += 16) {
+        const uint32_t word = cache_seen(m, k, i, c);
+        for (int x = 0; x < 32; ++x)
+          if (((word >> x) & 1u) != (sees(m, i, c + x, S) ? 1u : 0u)) ++failures;
+      }
+    }
     for (int parts : {1, 2, 3, 7})
       for (int chunk : {1, 4, 8}) {
         const int c = walk_chunk(w.n, parts, chunk), used = (w.n + c - 1) / c;
@@ -80,6 +89,18 @@ int main() {
   CacheMask f{0, big, 1, big, 1 << 28, make_udiv(big), make_udiv(1)};
   const RowKeys k = cache_row_keys(f, big - 1, big);
   if (k.lo != 0 || k.hi != big || k.pre != big) ++failures;
+  // dilations at and past the word's width
+  for (int dil : {31, 32, 33, 100, 1 << 28}) {
+    const CacheMask far{1, 0, dil, 0, 0, make_udiv(1), make_udiv(dil), cache_comb(dil)};
+    for (int i : {0, 31, 63, 200, 4095, big - 1}) {
+      const RowKeys rk = cache_row_keys(far, i, i + 1);
+      for (int c = i > 300 ? i - 300 : 0; c <= i; c += 16) {
+        const uint32_t word = cache_seen(far, rk, i, c);
+        for (int x = 0; x < 32; ++x)
+          if (((word >> x) & 1u) != (sees(far, i, c + x, i + 1) ? 1u : 0u)) ++failures;
+      }
+    }
+  }
   for (int bad : {-1, INT_MIN, 10, 11, INT_MAX})
     if (cache_page(bad, 10) != -1 || cache_slot(bad, 10) != -1) ++failures;
   for (int good : {0, 9})
