@@ -32,9 +32,10 @@ __device__ __forceinline__ T sel(int second, T a, T b) {
   return second ? b : a;
 }
 
-// x, hidden from the compiler: addresses made from it stay where they are used
+// x, hidden from the compiler: what is made from it stays where it is used
 // rather than in registers through the walk.
-__device__ __forceinline__ int here(int x) {
+template <class T>
+__device__ __forceinline__ T here(T x) {
   asm volatile("" : "+v"(x));
   return x;
 }
@@ -242,14 +243,20 @@ __global__ __launch_bounds__(256, 2) void cache_prompt_kernel(const CacheAttnPar
     // Score modifiers, in place; softmax in log2 units over kq.
     auto modify = [&](f32x16_t& s, int jb) __attribute__((always_inline)) {
       if constexpr (SCORE != CACHE_SOFTMAX) {
+        const float x0 = (float)(jb + 4 * here(lh) - ipos);
+        if (p.softcap > 0.f) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float v = __builtin_fmaf(sl, (float)(jb + 4 * lh + 8 * (e >> 2) + (e & 3) - ipos), s[e] * c1);
-          if (p.softcap > 0.f) {
+          for (int e = 0; e < 16; ++e) {
+            float v = __builtin_fmaf(sl, x0 + (float)(8 * (e >> 2) + (e & 3)), s[e] * c1);
             const float ex = __builtin_amdgcn_exp2f(v * (2.f * kCLog2e / p.softcap));
             v = p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + ex));
+            s[e] = SCORE == CACHE_SOFTMAX_MOD ? v * kCLog2e : v;
           }
-          s[e] = SCORE == CACHE_SOFTMAX_MOD ? v * kCLog2e : v;
+        } else {
+          constexpr float unit = SCORE == CACHE_SOFTMAX_MOD ? kCLog2e : 1.f;
+          const float c = here(c1) * unit, slope = here(sl) * unit;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(slope, x0 + (float)(8 * (e >> 2) + (e & 3)), s[e] * c);
         }
       }
     };
