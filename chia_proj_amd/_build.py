@@ -2,8 +2,8 @@
 
 The library is compiled with ``hipcc`` for gfx950 only and linked into the
 package directory, where :mod:`chia_proj_amd._lib` loads it with ctypes.  The
-three translation units compile in parallel (the two head-dim halves of the
-kernel instantiations and the C-ABI file).
+translation units (kernel instantiations by head dim, the C-ABI files) compile
+in parallel.
 """
 from __future__ import annotations
 

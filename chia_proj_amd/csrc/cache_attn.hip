@@ -152,8 +152,8 @@ Shape shape_of(const chia_cache_attn_args* a, const CacheMask& m) {
   Shape s;
   // 32 rows to a workgroup start and split better, 128 compute faster: about 870 and
   // 1700 (row x key)s per ns on a full chip, and 17 us more for the latter's longer steps
-  // (H32/8 D128, us with 32 and 128: one prompt of 300 tokens 17, 29; 8 of 48 over 4000: 70, 68;
-  // 32 of 32 over 4000: 134, 119; 64 of 10 over 4000, whose 40 rows fill 64 and 128: 145, 186).
+  // (H32/8 D128, us with 32 and 128: one prompt of 300 tokens 16, 25; 8 of 48 over 4000: 67, 60;
+  // 32 of 32 over 4000: 130, 108; 64 of 10 over 4000, whose 40 rows fill 64 and 128: 139, 156).
   const double each = (double)(t->batch * hkv) * (double)(t->seqlen < a->width * a->block_size ? t->seqlen : a->width * a->block_size);
   const double us32 = each * (double)((rows + 31) / 32 * 32) / 0.87e6, us128 = each * (double)((rows + 127) / 128 * 128) / 1.7e6 + 17.0;
   s.tile = rows <= 16 ? CACHE_ROWS16 : us32 <= us128 ? CACHE_ROWS32 : CACHE_ROWS128;
