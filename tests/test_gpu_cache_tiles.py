@@ -185,3 +185,16 @@ def test_gradients_are_refused():
         lib.attention_cache(q.requires_grad_(), kc, vc, ks, vs, table, lens)
     with torch.no_grad():
         lib.attention_cache(q, kc, vc, ks, vs, table, lens)
+
+
+@pytest.mark.parametrize("dilation", [2, 31, 32, 33, 100, 1 << 20])
+@pytest.mark.parametrize("causal", [True, False])
+def test_dilations_around_a_word(dilation, causal):
+    """The keys a row sees of 32 are one word: dilations below, at and past its width, on every row tile."""
+    _say(f"[dilation] {dilation} {causal}")
+    kw = dict(dilation=dilation, causal=causal)
+    c = Case([33, 700, 64, 301], H=8, Hkv=2, D=128, bs=16, seed=dilation)
+    c.check(c.call(**kw), **kw)
+    c = Case([33, 700, 64, 301], n=[20, 1, 0, 33], H=4, Hkv=2, D=64, dtype=E5, bs=32, seed=dilation + 1)
+    c.check(c.call(max_query=33, max_seqlen=700, **kw), **kw)
+    c.check(_prompt(c, **kw), **kw)
